@@ -3,7 +3,8 @@
 Loads libapus_gcuda.so (built in-tree by this folder's Makefile) with ctypes
 and exposes the entry points of include/apus_gcuda.h and
 include/apus_gmodel_gcuda.h with the reference's names and argument meaning
-(c/fp8blk.h, c/bf16.h, c/gmoe.h, c/gmtp.h).  There is no CPU fallback: if
+(c/fp8blk.h, c/bf16.h, c/gmoe.h, c/gmtp.h), and those of
+include/apus_attn_gcuda.h.  There is no CPU fallback: if
 the shared library is missing or fails to load, importing this module
 raises.
 """
@@ -195,6 +196,182 @@ apus_gspec_init = _fn("apus_gspec_init", None, _vp, _vp, _vp, _vp, _vp, _i, C.c_
 apus_gspec_free = _fn("apus_gspec_free", None, _vp)
 apus_gspec_prefill = _fn("apus_gspec_prefill", _i, _vp, _vp, _sz)
 apus_gspec_step = _fn("apus_gspec_step", _i, _vp, _vp, _i)
+
+
+# ---- batched attention and the 4-bit cache (include/apus_attn_gcuda.h) ------
+KV4_PAGE, KV4_GROUP = 64, 32
+
+
+class HeadRows(C.Structure):
+    """ApusHeadRows: BF16 rows of heads on the device."""
+    _fields_ = [("p", _vp), ("rows", _sz), ("heads", _sz), ("row_stride", _sz), ("head_stride", _sz)]
+
+
+class Kv4CacheDesc(C.Structure):
+    """ApusKv4Cache."""
+    _fields_ = [("pages", _vp), ("num_pages", _sz), ("heads", _sz), ("dim", _sz)]
+
+
+class Kv4BatchDesc(C.Structure):
+    """ApusKv4Batch."""
+    _fields_ = [("cu_rows", _vp), ("kv_len", _vp), ("page_table", _vp), ("table_stride", _sz), ("nseq", _sz),
+                ("max_rows", _sz), ("max_len", _sz)]
+
+
+class PromptBatchDesc(C.Structure):
+    """ApusPromptBatch."""
+    _fields_ = [("cu_q", _vp), ("cu_k", _vp), ("nseq", _sz), ("max_rows", _sz)]
+
+
+_rows_p, _kv4c_p, _kv4b_p = C.POINTER(HeadRows), C.POINTER(Kv4CacheDesc), C.POINTER(Kv4BatchDesc)
+_pb_p = C.POINTER(PromptBatchDesc)
+apus_gcuda_kv4_page_bytes = _fn("apus_gcuda_kv4_page_bytes", _sz, _sz, _sz)
+apus_gcuda_kv4_append_dev = _fn("apus_gcuda_kv4_append_dev", _i, _kv4c_p, _kv4b_p, _rows_p, _rows_p, _vp)
+apus_gcuda_kv4_read_dev = _fn("apus_gcuda_kv4_read_dev", _i, _kv4c_p, _kv4b_p, _rows_p, _rows_p, _vp)
+apus_gcuda_kv4_attn_workspace = _fn("apus_gcuda_kv4_attn_workspace", _sz, _kv4c_p, _kv4b_p, _sz)
+apus_gcuda_kv4_attn_dev = _fn("apus_gcuda_kv4_attn_dev", _i, _kv4c_p, _kv4b_p, _rows_p, _rows_p, _f, _vp, _sz, _sz,
+                              _vp, _sz, _vp)
+apus_gcuda_prompt_attn_dev = _fn("apus_gcuda_prompt_attn_dev", _i, _pb_p, _rows_p, _rows_p, _rows_p, _rows_p, _sz,
+                                 _f, _vp)
+
+
+def _same_device(what, dev, *tensors):
+    """Every tensor on the CUDA device `dev`, and that the current one."""
+    import torch
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise GcudaError(f"{what}: tensors on {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise GcudaError(f"{what}: tensors on {dev}, not on a GPU")
+    if dev.index != torch.cuda.current_device():
+        raise GcudaError(f"{what}: tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def head_rows(t, what="rows"):
+    """ApusHeadRows of a BF16 tensor [rows][heads][dim] (strided views too, the
+    dims contiguous)."""
+    import torch
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise GcudaError(f"{what}: BF16 [rows][heads][dim] with contiguous dims, not {t.dtype} {list(t.shape)} "
+                         f"with strides {t.stride()}")
+    return HeadRows(t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), t.stride(1))
+
+
+def _ints(what, t, dim):
+    import torch
+    if t.dtype != torch.int32 or t.dim() != dim or (t.numel() > 1 and t.stride(-1) != 1):
+        raise GcudaError(f"{what}: int32 with {dim} axes, contiguous, not {t.dtype} {list(t.shape)}")
+
+
+class Kv4Cache:
+    """A 4-bit key/value cache over `pages`, a contiguous uint8 tensor
+    [num_pages][heads][72 * dim] that the caller keeps (kv4_pages makes one)."""
+
+    def __init__(self, pages):
+        import torch
+        if pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous() or pages.shape[2] % 72:
+            raise GcudaError(f"kv4 cache: contiguous uint8 [pages][heads][72 * dim], not {pages.dtype} "
+                             f"{list(pages.shape)}")
+        self.pages, self.heads, self.dim = pages, pages.shape[1], pages.shape[2] // 72
+        self.desc = Kv4CacheDesc(pages.data_ptr(), pages.shape[0], self.heads, self.dim)
+        self.ref = C.pointer(self.desc)
+
+
+def kv4_pages(num_pages, heads, dim, device="cuda"):
+    """Zeroed pages of a 4-bit cache."""
+    import torch
+    n = apus_gcuda_kv4_page_bytes(heads, dim)
+    if not n:
+        check(-1, "kv4_pages")
+    return torch.zeros((num_pages, heads, n // heads), dtype=torch.uint8, device=device)
+
+
+class Kv4Batch:
+    """Sequences over a 4-bit cache (ApusKv4Batch): int32 device tensors
+    cu_rows [nseq + 1], kv_len [nseq] and page_table [nseq][pages], which the
+    kernels read when they run, and the host's bounds."""
+
+    def __init__(self, cu_rows, kv_len, page_table, max_rows, max_len):
+        _ints("cu_rows", cu_rows, 1)
+        _ints("kv_len", kv_len, 1)
+        _ints("page_table", page_table, 2)
+        n = kv_len.shape[0]
+        if cu_rows.shape[0] != n + 1 or page_table.shape[0] != n:
+            raise GcudaError(f"kv4 batch: {n} sequences, {cu_rows.shape[0]} row starts, {page_table.shape[0]} page lists")
+        self.tensors = (cu_rows, kv_len, page_table)
+        self.desc = Kv4BatchDesc(cu_rows.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+                                 page_table.stride(0) if n > 1 else page_table.shape[1], n, max_rows, max_len)
+        self.ref = C.pointer(self.desc)
+
+
+class PromptBatch:
+    """Packed prompts (ApusPromptBatch): int32 device tensors cu_q, cu_k
+    [nseq + 1]; cu_k = cu_q for whole prompts."""
+
+    def __init__(self, cu_q, cu_k, max_rows):
+        _ints("cu_q", cu_q, 1)
+        _ints("cu_k", cu_k, 1)
+        if cu_q.shape != cu_k.shape or cu_q.shape[0] < 1:
+            raise GcudaError(f"prompt batch: {cu_q.shape[0]} and {cu_k.shape[0]} row starts")
+        self.tensors = (cu_q, cu_k)
+        self.desc = PromptBatchDesc(cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, max_rows)
+        self.ref = C.pointer(self.desc)
+
+
+def _kv4_call(what, cache, batch, dim_of, *more):
+    for t in dim_of:
+        if t.shape[-1] != cache.dim:
+            raise GcudaError(f"{what}: head dim {t.shape[-1]}, the cache's is {cache.dim}")
+    _same_device(what, cache.pages.device, *batch.tensors, *dim_of, *more)
+
+
+def kv4_append(cache, batch, k, v, stream=None):
+    """Quantise the batch's rows k, v [rows][heads][dim] into the cache."""
+    _kv4_call("kv4_append", cache, batch, (k, v))
+    check(apus_gcuda_kv4_append_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"), stream_of(stream)),
+          "kv4_append")
+
+
+def kv4_read(cache, batch, k, v, stream=None):
+    """Read the batch's rows back into k, v [rows][heads][dim]."""
+    _kv4_call("kv4_read", cache, batch, (k, v))
+    check(apus_gcuda_kv4_read_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"), stream_of(stream)),
+          "kv4_read")
+
+
+def kv4_attn_workspace(cache, batch, q_heads):
+    """Bytes of workspace that kv4_attn needs for the batch (0: none)."""
+    apus_gcuda_clear_error()
+    n = apus_gcuda_kv4_attn_workspace(cache.ref, batch.ref, q_heads)
+    if not n and apus_gcuda_last_error():
+        check(-1, "kv4_attn_workspace")
+    return n
+
+
+def kv4_attn(cache, batch, q, out, scale, workspace=None, sel=None, pool=0, stream=None):
+    """Attention of q [rows][q_heads][dim] over the cache into out; sel: uint8
+    [rows][pools], the pools of `pool` positions that each row keeps."""
+    import torch
+    _kv4_call("kv4_attn", cache, batch, (q, out), workspace, sel)
+    if sel is not None and (sel.dtype != torch.uint8 or sel.dim() != 2 or sel.shape[0] < q.shape[0] or
+                            not sel.is_contiguous()):
+        raise GcudaError(f"kv4_attn: sel is contiguous uint8 [rows][pools], not {sel.dtype} {list(sel.shape)}")
+    check(apus_gcuda_kv4_attn_dev(cache.ref, batch.ref, head_rows(q, "q"), head_rows(out, "out"), scale,
+                                  None if sel is None else sel.data_ptr() or cache.pages.data_ptr(),
+                                  0 if sel is None else sel.shape[1], pool,
+                                  None if workspace is None else workspace.data_ptr(),
+                                  0 if workspace is None else workspace.numel() * workspace.element_size(),
+                                  stream_of(stream)), "kv4_attn")
+
+
+def prompt_attn(batch, q, k, v, out, scale, stream=None):
+    """Causal attention over packed prompts: q, out [rows][q_heads][dim],
+    k, v [keys][heads][dim]."""
+    if not q.shape[-1] == k.shape[-1] == v.shape[-1] == out.shape[-1]:
+        raise GcudaError(f"prompt_attn: head dims {[t.shape[-1] for t in (q, k, v, out)]}")
+    _same_device("prompt_attn", q.device, k, v, out, *batch.tensors)
+    check(apus_gcuda_prompt_attn_dev(batch.ref, head_rows(q, "q"), head_rows(k, "k"), head_rows(v, "v"),
+                                     head_rows(out, "out"), q.shape[-1], scale, stream_of(stream)), "prompt_attn")
 
 
 EP_HANDLE_BYTES = 64   # sizeof(cudaIpcMemHandle_t)

@@ -1,0 +1,38 @@
+// attn_dev.h — what the translation units of include/apus_attn_gcuda.h share:
+// the host's checks of arguments, and the device error word.
+#pragma once
+#include "gcuda.h"
+#include "kv4_layout.h"
+#include "../../include/apus_attn_gcuda.h"
+
+static_assert(KV4_PAGE == APUS_KV4_PAGE && KV4_GROUP == APUS_KV4_GROUP, "public and internal layout");
+
+enum { ATTN_ERR_PAGE = 41, ATTN_ERR_SEQ = 42, ATTN_ERR_WAIT = 43 };   // 43..: a bounded wait gave up
+
+// Device views of the public structs (sizes checked to fit ints).
+struct Kv4View {
+    uint8_t *pages;
+    long num_pages;
+    int heads, dim;
+    const int32_t *cu, *len, *table;
+    long table_stride;
+    int nseq;
+    int rows;                 // row capacity of the row arrays
+    int max_rows, max_len;
+};
+struct RowsView {
+    uint16_t *p;
+    long rs, hs;              // row and head strides
+};
+
+// Argument checks (attn_check.cu); each records the reason and returns -1.
+int attn_check_rows(const char *what, const ApusHeadRows *r, size_t dim, bool output);
+int attn_check_dim(const char *what, size_t dim);
+int kv4_check(const char *what, const ApusKv4Cache *c, const ApusKv4Batch *b, size_t rows, Kv4View *out);
+static inline RowsView rows_view(const ApusHeadRows *r) {
+    return RowsView{r->p, (long)r->row_stride, (long)r->head_stride};
+}
+// the device error words
+int kv4_cache_error_read_and_clear(void);
+int kv4_attn_error_read_and_clear(void);
+int prompt_attn_error_read_and_clear(void);

@@ -9,6 +9,7 @@
 
 #include "gcuda.h"
 #include "../../include/apus_gcuda.h"
+#include "attn_dev.h"
 
 static thread_local char g_err[512];
 
@@ -248,7 +249,10 @@ void apus_gcuda_clear_error(void) { g_err[0] = 0; }
 int apus_gcuda_kernel_error(void) {
     cudaDeviceSynchronize();
     const int a = kernel_error_read_and_clear(), b = ep_error_read_and_clear(), c = tc_error_read_and_clear();
-    return a ? a : (b ? b : c);
+    if (a || b || c) return a ? a : (b ? b : c);
+    const int k = kv4_cache_error_read_and_clear(), l = kv4_attn_error_read_and_clear(),
+              p = prompt_attn_error_read_and_clear();
+    return k ? k : (l ? l : p);
 }
 
 int apus_gcuda_register_region(const void *ptr, size_t len) {
