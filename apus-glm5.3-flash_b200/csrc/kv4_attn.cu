@@ -14,26 +14,38 @@
 //
 // Bound: HBM at long contexts (a position of a head is 9/8 dim bytes), with
 // the unpacking of the codes close behind it, so the unpacking is what the
-// layout serves.  mma.sync m16n8k16 with the cached positions (scores) or the
-// dims (output) as its 16 rows and the query columns (rows of the step times
-// heads of the group) as its 8: tcgen05 needs 64 rows of a tile at least and
-// operands in shared memory, so the codes would have to be unpacked into it
-// first, and at 1 to 16 columns its rate buys nothing.
-//   * Key codes 0-15 enter as f16 subnormals: a 4-bit field at bits 0-3 or
-//     4-7 of a half is c 2^-24 or c 2^-20 as it stands, so one AND unpacks two
-//     codes.  The factor 16 goes into the query's fragments, the offset 8 into
-//     the accumulator's start, -8 sum q, and 2^24 into the column's scale.
+// layout serves.  mma.sync with the query columns (rows of the step times
+// heads of the group) in tiles of 8: tcgen05 needs 64 rows of a tile at least
+// and operands in shared memory, so the codes would have to be unpacked into
+// it first, and at 1 to 16 columns its rate buys nothing.
+//   * m16n8k16 on f16 with the positions (scores) or the dims (output) as its
+//     16 rows and the query columns as its 8.  The other way round the weights
+//     would need no transpose, but half the rows would idle and their zeros cost
+//     a register each (measured: 372 instructions for 16 positions of dim 128).
+//   * Key codes 0-15 enter as f16 subnormals: a field at bits 0-3 or 4-7 of a
+//     half is c 2^-24 or c 2^-20 as it stands, so one AND unpacks two codes.  The
+//     factor 16 goes into the query's fragments, the offset 8 is taken off the
+//     sum, and 2^24 goes into the column's scale.
 //   * Value codes of two positions are paired by one byte permute, OR-ed into
-//     the mantissa of 128.0 (BF16) and 136 is subtracted: exact integers.
-//   * Weights stay fp32 up to the product with the value's scale; p and p r are
-//     rounded to BF16 (2^-9 each, any range; f16 would lose small scales).
+//     the mantissa of 1024 and the offset is subtracted: exact integers.
+//   * Scales are unpacked once a unit, not once a lane that needs them: fp32 for
+//     the keys; for the values f16 below 2, with a power of two a position that
+//     goes into the weight's exponent.  Two f16 roundings (2^-12) a weight.
+// (E4M3 mma.sync looks four times as fast but is carried out as conversions and
+// f16 products: 50 conversions for 16 positions of dim 128, and no faster.)
 //
-// Work: a CTA of four warps takes a chunk of one sequence's positions for one
-// cache head and 8 NT columns.  Every warp streams its own units of U
-// positions through its own two stages (bulk copies of whole cache blocks, an
-// mbarrier each) with its own maximum, sum and output tile, so the loop has no
-// CTA barrier; the warps are joined once at the end.  Chunks are joined by a
-// second kernel when a sequence has several.
+// Work: a segment is one sequence's positions for one cache head and 8 NT
+// columns.  All segments' pages in a row are cut into equal runs, one a CTA,
+// one wave of CTAs (lengths are read on the device, so ragged batches balance
+// too); a segment that a cut divides is put together by a second kernel.
+// Inside a CTA four warps each stream units of U positions of their own
+// through two stages of their own with their own maximum, sum and output
+// tile, so the loop has no CTA barrier; the warps are joined once a segment.
+// Units come by cp.async, nine 16-byte pieces a lane: bulk copies of one or four
+// pieces a unit cost their issuing warp about 250 cycles each, as much as two
+// fragments' work.  Under a selection the positions that any of the columns keeps
+// are listed and gathered row by row, so what no column keeps is neither read
+// nor computed.
 #include <type_traits>
 
 #include "attn_dev.h"
@@ -46,15 +58,22 @@ __device__ int g_kv4a_err;   // attn_dev.h's codes
 
 namespace kv4 {
 constexpr int WARPS = 4, THREADS = 32 * WARPS, STAGES = 2;
-// Positions of a unit: one page where a page is at most 9 KB, half a page of
-// dim 256, so that two stages of four warps leave room for three CTAs an SM.
+// CTAs an SM holds: as many as the registers allow (168 and 255 a thread).
+constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }
+// Positions of a unit: 4608 bytes of cache.
 template <int D> struct Cfg {
-    static constexpr int U = D == 256 ? 32 : 64;
+    static constexpr int U = 4096 / D;
     static constexpr int NG = D / 32;                       // scale groups
     static constexpr int KC = 0, VC = U * D / 2, KS = U * D, VS = KS + U * NG * 2;
     static constexpr int STAGE = VS + U * NG * 2;           // 72 D U / 64
-    static constexpr int SMEM = WARPS * STAGES * STAGE;
+    // a unit's scales as the loop wants them: keys' fp32 [U][NG], values' f16
+    // pairs of positions, and each position's power of two with its inverse
+    static constexpr int KF = STAGES * STAGE, VH = KF + U * NG * 4, PW = VH + U * NG * 2;
+    static constexpr int WARP_SMEM = PW + U * 8;
+    static constexpr int SMEM = WARPS * WARP_SMEM;
+    static constexpr int LIST = 2048;                       // selected positions at a time (16-bit offsets)
 };
+constexpr int LIST_SPAN = 32768;                            // positions that one list can cover
 constexpr float NEG_INF = -__builtin_huge_valf();
 }  // namespace kv4
 
@@ -62,29 +81,42 @@ struct Kv4AttnArgs {
     Kv4View v;
     RowsView q, out;
     int group;                // query heads of a cache head
+    uint64_t group_magic;     // ceil(2^40 / group): c / group = c * magic >> 40 (a column and a head are below 2^20, 2^16)
     float zscale;             // scale * log2(e)
     const uint8_t *sel;
     long sel_stride;
     int pool;
     uint64_t pool_magic;      // ceil(2^36 / pool): j / pool = j * magic >> 36 for j < 2^28, pool <= 128
-    int chunk_pos, nchunk, ncb;
-    float *part;
+    int whole;                // no segment is cut: a page of work stands for a segment
+    int min_pages;            // pages of a run at least
+    long *plan;               // workspace: runs, pages in all, first page of each sequence
+    float *part;              // workspace: two partial results a CTA
 };
 
+// Quotients without the long way round of 64-bit division where they fit 32.
+APUS_DEV long div_long(long a, long b) {
+    return ((unsigned long)(a | b) >> 32) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+APUS_DEV int row_of(const Kv4AttnArgs &a, int c) { return (int)(((uint64_t)(uint32_t)c * a.group_magic) >> 40); }
+
+constexpr int KJ_RUNS = 148 * 4;          // runs at most (a multiple of 4)
+
+// The work: sequence s has heads * ncb segments of `pages` pages (one at
+// least, so that a row that sees nothing is written too).
+struct Kv4Work { Kv4Seq sq; int ncb; long pages; };
+APUS_DEV Kv4Work kv4_work(const Kv4AttnArgs &a, int s, int cols_block) {
+    Kv4Work w;
+    w.sq = kv4_seq(a.v.cu[s], a.v.cu[s + 1], a.v.len[s], a.v.rows, a.v.max_rows, a.v.max_len);
+    w.ncb = (w.sq.n * a.group + cols_block - 1) / cols_block;
+    w.pages = a.whole ? 1 : max(1, (w.sq.len + KV4_PAGE - 1) / KV4_PAGE);
+    return w;
+}
+
+// c += a . b
 APUS_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-APUS_DEV void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-APUS_DEV uint32_t movmatrix(uint32_t a) {
-    uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-    return d;
 }
 APUS_DEV uint32_t pack_bf16(float lo, float hi) {
     uint32_t d;
@@ -96,28 +128,78 @@ APUS_DEV uint32_t pack_f16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
-APUS_DEV uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-// All ones in each half whose sign bit is set.
-APUS_DEV uint32_t sign_bf16x2(uint32_t x) {
-    uint32_t d;
-    asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(d) : "r"(x));
-    return d;
+// cp.async of 4, 8 or 16 bytes.
+template <int N> APUS_DEV void cp_async_n(void *dst, const void *src) {
+    if constexpr (N == 16) cp_async16(dst, src);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(N) : "memory");
 }
 APUS_DEV float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// The low four bits of each half as the BF16 integers code - 8.
-APUS_DEV uint32_t code_bf16x2(uint32_t x) {
-    const uint32_t u = (x & 0x000f000fu) | 0x43004300u;      // 128 + code
+// 8x8 transpose of f16 pairs across the warp.
+APUS_DEV uint32_t movmatrix(uint32_t a) {
     uint32_t d;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(u), "r"(0x43084308u));
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+APUS_DEV uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// All ones in each half whose sign bit is set.
+APUS_DEV uint32_t sign_x2(uint32_t x) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(d) : "r"(x));
+    return d;
+}
+// Constants of the code unpacking, kept in registers: an instruction takes one
+// immediate, and the compiler would split (x & mask) | magic in two.
+struct CodeConst { uint32_t lo, hi, magic, scale, off; };
+APUS_DEV CodeConst code_const() {
+    CodeConst k;
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(k.lo));
+    asm volatile("mov.b32 %0, 0x00f000f0;" : "=r"(k.hi));
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(k.magic));
+    asm volatile("mov.b32 %0, 0x2c002c00;" : "=r"(k.scale));
+    asm volatile("mov.b32 %0, 0xd480d480;" : "=r"(k.off));
+    return k;
+}
+// Bits 0-3 (4-7) of each half as the f16 integers code - 8: OR-ed into the
+// mantissa of 1024 the code counts 1 (16), and the rest is exact.
+APUS_DEV uint32_t code_lo(uint32_t x, const CodeConst &k) {
+    uint32_t u, d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(x), "r"(k.lo), "r"(k.magic));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(u), "r"(0x64086408u));
+    return d;
+}
+APUS_DEV uint32_t code_hi(uint32_t x, const CodeConst &k) {
+    uint32_t u, d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(u) : "r"(x), "r"(k.hi), "r"(k.magic));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(u), "r"(k.scale), "r"(k.off));
+    return d;
+}
+template <int N> APUS_DEV void lds_floats(float (&f)[N], const float *p) {
+    if constexpr (N == 2) { const float2 t = *(const float2 *)p; f[0] = t.x; f[1] = t.y; }
+    else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 t = *(const float4 *)(p + i);
+            f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
+        }
+    }
+}
+template <int N> APUS_DEV void lds_pairs(uint32_t (&w)[N], const uint32_t *p) {
+    if constexpr (N == 2) { const uint2 t = *(const uint2 *)p; w[0] = t.x; w[1] = t.y; }
+    else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 t = lds128(p + i);
+            w[i] = t.x; w[i + 1] = t.y; w[i + 2] = t.z; w[i + 3] = t.w;
+        }
+    }
 }
 template <int N> APUS_DEV void lds_words(uint32_t (&w)[N], const uint8_t *p) {
     if constexpr (N == 1) w[0] = *(const uint32_t *)p;
@@ -125,133 +207,105 @@ template <int N> APUS_DEV void lds_words(uint32_t (&w)[N], const uint8_t *p) {
     else { const uint4 t = lds128(p); w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kv4::THREADS, NT == 1 ? 3 : 2) k_kv4_attn(const Kv4AttnArgs a) {
+template <int D, int NT, bool SEL>
+__global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(const Kv4AttnArgs a) {
     using C = kv4::Cfg<D>;
-    constexpr int NG = C::NG, U = C::U, SUB = U / 16, COLS = 8 * NT, UPP = KV4_PAGE / U;
+    constexpr int NG = C::NG, U = C::U, COLS = 8 * NT, UPP = KV4_PAGE / U;
     constexpr float NEG_INF = kv4::NEG_INF;
     extern __shared__ __align__(128) uint8_t kv4_dyn[];
-    __shared__ __align__(8) uint64_t full[kv4::WARPS][kv4::STAGES];
-    __shared__ int abort_flag;
     __shared__ float join_m[kv4::WARPS][COLS], join_l[kv4::WARPS][COLS];
+    __shared__ long scan_s[kv4::WARPS];
+    __shared__ long found_s[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-    const int chunk = blockIdx.x, head = (int)(blockIdx.y / (unsigned)a.ncb), cb = (int)(blockIdx.y % (unsigned)a.ncb);
-    const int seq = blockIdx.z;
 
-    const Kv4Seq sq = kv4_seq(a.v.cu[seq], a.v.cu[seq + 1], a.v.len[seq], a.v.rows, a.v.max_rows, a.v.max_len);
-    if (sq.bad && threadIdx.x == 0) atomicExch(&g_kv4a_err, (int)ATTN_ERR_SEQ);
+    // ---- this CTA's run of pages [x, xe)
+    pdl_launch_dependents();
+    // weights of the sequences, THREADS at a time: this thread's, the pages
+    // before it and (through `before`) those of all
+    auto scan = [&](int s0, long &w, long &before) -> long {
+        const int s = s0 + threadIdx.x;
+        w = 0;
+        if (s < a.v.nseq) {
+            const Kv4Work k = kv4_work(a, s, COLS);
+            if (k.sq.bad && blockIdx.x == 0) atomicExch(&g_kv4a_err, (int)ATTN_ERR_SEQ);
+            w = (long)a.v.heads * k.ncb * k.pages;
+        }
+        long incl = w;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += o;
+        }
+        if (lane == 31) scan_s[warp] = incl;
+        __syncthreads();
+        long at = before + incl - w;
+        for (int k = 0; k < kv4::WARPS; k++) {
+            if (k < warp) at += scan_s[k];
+            before += scan_s[k];
+        }
+        __syncthreads();
+        return at;
+    };
+    long total = 0, w0 = 0, at0 = 0;
+    for (int s0 = 0; s0 < a.v.nseq; s0 += kv4::THREADS) at0 = scan(s0, w0, total);
+    const long runs = min((long)gridDim.x, max(1l, div_long(total, a.min_pages)));
+    if (blockIdx.x >= runs && blockIdx.x != 0) return;
+    long x = div_long(total * blockIdx.x, runs);
+    const long xe = div_long(total * (blockIdx.x + 1), runs);
+    // the sequence in which it begins, and that sequence's first page
+    long before = 0;
+    for (int s0 = 0; s0 < a.v.nseq; s0 += kv4::THREADS) {
+        if (a.v.nseq > kv4::THREADS) at0 = scan(s0, w0, before);
+        const int s = s0 + threadIdx.x;
+        if (s < a.v.nseq && w0 && at0 <= x && x < at0 + w0) { found_s[0] = s; found_s[1] = at0; }
+        if (blockIdx.x == 0 && a.plan && s < a.v.nseq) a.plan[2 + s] = at0;
+    }
+    if (blockIdx.x == 0 && a.plan && threadIdx.x == 0) { a.plan[0] = runs; a.plan[1] = total; }
+    if (x >= xe) return;
+    __syncthreads();
+    int seq = (int)found_s[0];
+    long seq_x = found_s[1];
+    uint8_t *const own = kv4_dyn + warp * C::WARP_SMEM, *const stages = own;
+    uint16_t *list = (uint16_t *)(kv4_dyn + C::SMEM);
+    __shared__ int wcount[kv4::WARPS];
+
+    while (x < xe) {
+    // ---- the next piece: pages pg0 .. pg1 of one segment
+    Kv4Work wk = kv4_work(a, seq, COLS);
+    while (x >= seq_x + (long)a.v.heads * wk.ncb * wk.pages) {
+        seq_x += (long)a.v.heads * wk.ncb * wk.pages;
+        wk = kv4_work(a, ++seq, COLS);
+    }
+    const Kv4Seq sq = wk.sq;
+    const int seg = (int)div_long(x - seq_x, wk.pages);
+    const long seg_x = seq_x + seg * wk.pages;
+    const int head = wk.ncb == 1 ? seg : seg / wk.ncb, cb = seg - head * wk.ncb;
+    const long piece_e = min(xe, seg_x + wk.pages);
+    const bool starts = x == seg_x, ends = piece_e == seg_x + wk.pages;
     const int cols = sq.n * a.group, c0 = cb * COLS;
-    if (c0 >= cols) return;
     const int cend = min(c0 + COLS, cols);
     // the positions that the first and the last row of the block see
     const int lim_row0 = sq.len - sq.n + 1;
-    const int lim0 = lim_row0 + c0 / a.group, lim1 = lim_row0 + (cend - 1) / a.group;
-    const int p0 = chunk * a.chunk_pos, p1 = min(p0 + a.chunk_pos, lim1);
-    if (p0 >= p1 && a.nchunk > 1) return;      // the joining kernel knows it too
+    const int lim0 = lim_row0 + row_of(a, c0), lim1 = lim_row0 + row_of(a, cend - 1);
+    const int p0 = a.whole ? 0 : (int)(x - seg_x) * KV4_PAGE;
+    const int p1 = a.whole ? lim1 : min((int)(piece_e - seg_x) * KV4_PAGE, lim1);
+    const int32_t *table = a.v.table + (long)seq * a.v.table_stride;
 
-    if (threadIdx.x == 0) {
-        for (int w = 0; w < kv4::WARPS; w++)
-            for (int s = 0; s < kv4::STAGES; s++) mbar_init(&full[w][s], 1);
-        abort_flag = 0;
-        fence_barrier_init();
+    // the query rows of this lane's columns, on their way while the first units are fetched
+    uint4 raw[NT][NG];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int c = c0 + nt * 8 + g, t = row_of(a, min(c, cols - 1));
+        const uint16_t *qp = a.q.p + (long)(sq.row0 + t) * a.q.rs + (long)(head * a.group + min(c, cols - 1) - t * a.group) * a.q.hs;
+#pragma unroll
+        for (int j = 0; j < NG; j++)
+            raw[nt][j] = c < cols ? *(const uint4 *)(qp + 32 * j + 8 * q4) : make_uint4(0, 0, 0, 0);
     }
-    // ---- this block's units: all of them, or those an indexer kept something in
-    const int units_all = p1 > p0 ? (p1 - p0 + U - 1) / U : 0;
-    uint16_t *list = (uint16_t *)(kv4_dyn + C::SMEM);
-    __shared__ int list_n;
-    if (a.sel) {
-        if (threadIdx.x == 0) list_n = 0;
-        __syncthreads();
-        // a unit counts when a row of the block sees one of its positions
-        for (int u0 = 0; u0 < units_all; u0 += kv4::THREADS) {
-            const int u = u0 + threadIdx.x;
-            bool any = false;
-            if (u < units_all) {
-                const int b = p0 + u * U, e = min(b + U, p1);
-                const long q0 = b / a.pool, q1 = min((long)((e - 1) / a.pool) + 1, a.sel_stride);
-                for (int t = c0 / a.group; t <= (cend - 1) / a.group && !any; t++) {
-                    const int lim = lim_row0 + t;
-                    if (lim <= b) continue;
-                    any = e > lim - lim % a.pool;
-                    const uint8_t *sr = a.sel + (long)(sq.row0 + t) * a.sel_stride;
-                    for (long i = q0; i < q1; i++) any |= sr[i] != 0;
-                }
-            }
-            // kept in order: the sums do not depend on timing
-            const unsigned bal = __ballot_sync(0xffffffffu, any);
-            __shared__ int wcount[kv4::WARPS];
-            if (lane == 0) wcount[warp] = __popc(bal);
-            __syncthreads();
-            int at = list_n;
-            for (int w = 0; w < warp; w++) at += wcount[w];
-            if (any) list[at + __popc(bal & ((1u << lane) - 1))] = (uint16_t)u;
-            __syncthreads();
-            if (threadIdx.x == 0)
-                for (int w = 0; w < kv4::WARPS; w++) list_n += wcount[w];
-            __syncthreads();
-        }
-    } else {
-        __syncthreads();
-    }
-    const int units = a.sel ? list_n : units_all;
-    volatile int *ab = &abort_flag;
-
-    // ---- the query's fragments: column g of each n tile, dims in the order in
-    // which a lane meets the key codes (dim 8 q4 + i of a group is code i)
+    // the query's fragments, the columns' offsets, factors and limits (below)
     uint32_t Q[NT][NG][4];
     float cinit[NT][NG][2], fac[NT][2];
     int lim[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int c = c0 + nt * 8 + g;
-        const bool on = c < cols;
-        const uint16_t *qp = a.q.p + (long)(sq.row0 + (on ? c / a.group : 0)) * a.q.rs +
-                             (long)(head * a.group + (on ? c % a.group : 0)) * a.q.hs;
-        uint4 raw[NG];
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            raw[j] = on ? *(const uint4 *)(qp + 32 * j + 8 * q4) : make_uint4(0, 0, 0, 0);
-            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-        }
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // a power of two that brings the largest magnitude to [2^14, 2^15): f16
-        // holds every BF16 within 2^-28 of it exactly, smaller ones to 2^-39 of it
-        const int e = top ? max((int)(top >> 7) - 127, -100) : 0;
-        const float up = __int_as_float((127 + 14 - e) << 23);
-        const float f = a.zscale * __int_as_float((127 + e - 14) << 23) * 16777216.0f;
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            const float x[8] = {bf16lo(raw[j].x), bf16hi(raw[j].x), bf16lo(raw[j].y), bf16hi(raw[j].y),
-                                bf16lo(raw[j].z), bf16hi(raw[j].z), bf16lo(raw[j].w), bf16hi(raw[j].w)};
-            float qs = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float down = (i & 1) ? up * 0.0625f : up;    // codes in the high nibbles stand 16 times higher
-                const uint32_t h = pack_f16(x[i] * down, x[i + 4] * down);
-                Q[nt][j][i] = h;
-                const float2 back = __half22float2(*(const __half2 *)&h);
-                qs += (back.x + back.y) * ((i & 1) ? 16.0f : 1.0f);
-            }
-            qs += __shfl_xor_sync(0xffffffffu, qs, 1);
-            qs += __shfl_xor_sync(0xffffffffu, qs, 2);
-            qs *= -8.0f / 16777216.0f;                             // the codes' offset
-            cinit[nt][j][0] = __shfl_sync(0xffffffffu, qs, 8 * q4);
-            cinit[nt][j][1] = __shfl_sync(0xffffffffu, qs, 8 * q4 + 4);
-        }
-        fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * q4);
-        fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * q4 + 4);
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int cc = min(c0 + nt * 8 + 2 * q4 + u, cols - 1);
-            lim[nt][u] = lim_row0 + cc / a.group;
-        }
-    }
-
-    float O[NT][D / 16][4], m[NT][2], l[NT][2];
+    float O[NT][D / 16][4], m[NT][2], l[NT][2];      // columns 2 q4, 2 q4 + 1; l: this lane's positions
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -262,110 +316,102 @@ __global__ void __launch_bounds__(kv4::THREADS, NT == 1 ? 3 : 2) k_kv4_attn(cons
         l[nt][0] = l[nt][1] = 0.f;
     }
 
-    // ---- this warp's units warp, warp + WARPS, ...: lane i holds the page of
-    // the i-th of the next 32
-    const int mine = units > warp ? (units - warp + kv4::WARPS - 1) / kv4::WARPS : 0;
-    uint8_t *stages = kv4_dyn + warp * kv4::STAGES * C::STAGE;
-    const int32_t *table = a.v.table + (long)seq * a.v.table_stride;
-    int my_unit = 0, my_page = -1;
-    auto fetch_ids = [&](int i0) {     // units i0 .. i0 + 31 of this warp
-        const int i = i0 + lane;
-        my_page = -1;
-        if (i < mine) {
-            const int u = warp + i * kv4::WARPS;
-            my_unit = a.sel ? list[u] : u;
-            const int page = table[(p0 + my_unit * U) / KV4_PAGE];
-            if (kv4_page_ok(page, a.v.num_pages)) my_page = page;
-            else atomicExch(&g_kv4a_err, (int)ATTN_ERR_PAGE);
-        }
-    };
-    struct Unit { int page, u; };
-    auto load = [&](int i) -> Unit {   // unit i of this warp into stage i % STAGES (whole warp)
-        if (i >= mine) return Unit{-1, 0};
-        if ((i & 31) == 0) fetch_ids(i);
-        const int page = __shfl_sync(0xffffffffu, my_page, i & 31), u = __shfl_sync(0xffffffffu, my_unit, i & 31);
-        if (lane == 0) {
-            uint64_t *bar = &full[warp][i % kv4::STAGES];
-            uint8_t *dst = stages + (i % kv4::STAGES) * C::STAGE;
-            if (page >= 0) {
-                const uint8_t *src = a.v.pages + kv4_block_at(page, head, a.v.heads, D);
-                mbar_arrive_expect_tx(bar, C::STAGE);
-                if (UPP == 1) {
-                    bulk_g2s(dst, src, C::STAGE, bar);
-                } else {
-                    const int h = (p0 / U + u) % UPP;
-                    bulk_g2s(dst + C::KC, src + h * (U * D / 2), U * D / 2, bar);
-                    bulk_g2s(dst + C::VC, src + kv4_v_codes(D) + h * (U * D / 2), U * D / 2, bar);
-                    bulk_g2s(dst + C::KS, src + kv4_k_scales(D) + h * (U * NG * 2), U * NG * 2, bar);
-                    bulk_g2s(dst + C::VS, src + kv4_v_scales(D) + h * (U * NG * 2), U * NG * 2, bar);
-                }
-            } else {
-                mbar_arrive(bar);      // no page: nothing to read, the unit is left out
-            }
-        }
-        return Unit{page, u};
-    };
-
-    // the cached position of row r of a 16-row fragment: rows 2 q, 2 q + 1 are
-    // positions q, 4 + (q ^ 1), so that the quads of one shared-memory access
-    // fall in different banks for keys and for values
+    // the cached position of place r of a 16-position fragment: places 2 q,
+    // 2 q + 1 are positions q, 4 + (q ^ 1), so that the quads of one
+    // shared-memory access fall in different banks for keys and for values
     const int pg = (g & 1) ? 4 + ((g >> 1) ^ 1) : (g >> 1), vp1 = 4 + (q4 ^ 1);
 
-    auto process = [&](const uint8_t *st, int pos0, auto masked_t) {
-        constexpr bool MASKED = decltype(masked_t)::value;
-        float z[NT][SUB][4];
-        // ---- scores
+    const CodeConst cc = code_const();
+    // A unit's scales as the loop below wants them.  A position's value scales
+    // are 2^E times numbers below 2, exact in f16 (those below 2^-24 of the
+    // largest become 0); E is -112 at least, so that 2^-E stays finite.  Whole
+    // warp; a lane takes four scales of each kind.
+    auto prepare = [&](const uint8_t *st) {
+        static_assert(U * NG == 128, "four scales of keys and of values a lane");
+        const uint2 k = *(const uint2 *)(st + C::KS + lane * 8), v = *(const uint2 *)(st + C::VS + lane * 8);
+        *(float4 *)(own + C::KF + lane * 16) = make_float4(bf16lo(k.x), bf16hi(k.x), bf16lo(k.y), bf16hi(k.y));
+        const float vf[4] = {bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y)};
+        float top[2];                              // largest scale of this lane's position (NG 2: two)
+        top[0] = fmaxf(vf[0], vf[1]);
+        top[1] = fmaxf(vf[2], vf[3]);
+        if constexpr (NG > 2) {
+            top[0] = fmaxf(top[0], top[1]);
+            if constexpr (NG == 8) top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], 1));
+            top[1] = top[0];
+        }
+        float inv[2];
 #pragma unroll
-        for (int sub = 0; sub < SUB; sub++) {
-            const int ra = sub * 16 + pg;
+        for (int u = 0; u < (NG == 2 ? 2 : 1); u++) {
+            int e = (int)(__float_as_uint(top[u]) >> 23) - 127;    // a NaN's or an infinity's scales stay what they are
+            e = max(min(e, 120), -112);
+            inv[u] = __int_as_float((127 - e) << 23);
+            const int r = NG == 2 ? 2 * lane + u : lane / (NG / 4);
+            *(float2 *)(own + C::PW + r * 8) = make_float2((float)e, inv[u]);
+        }
+        if constexpr (NG > 2) inv[1] = inv[0];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = (lane * 4 + i) / NG, j = (lane * 4 + i) % NG, e = (r >> 2) & 1;
+            const int at = (((r >> 3) * 4 + ((r & 3) ^ e)) * NG + j) * 2 + e;
+            ((__half *)(own + C::VH))[at] = __float2half_rn(vf[i] * inv[i >> 1]);
+        }
+        __syncwarp();
+    };
+
+    // 16 positions at place `at` of a stage: the positions from pos0 on, or (SEL)
+    // those that the list names, n of them
+    auto process = [&](const uint8_t *st, int at, int pos0, const uint16_t *names, int n, auto masked_t) {
+        constexpr bool MASKED = decltype(masked_t)::value;
+        float z[NT][4];                // positions pg (0, 1), pg + 8 (2, 3); columns 2 q4 (0, 2), 2 q4 + 1
+        float2 pw[2];                  // their powers of two
+        {
             uint32_t wa[NG], wb[NG];
             constexpr int JB = NG < 4 ? NG : 4;
 #pragma unroll
             for (int h = 0; h < NG / JB; h++) {
                 uint32_t ta[JB], tb[JB];
-                const int off = kv4_k_word(D, pg, h * JB, q4) * 4;
-                lds_words<JB>(ta, st + C::KC + ra * (D / 2) + off);
-                lds_words<JB>(tb, st + C::KC + (ra + 8) * (D / 2) + off);
+                const uint8_t *kp = st + C::KC + (at + pg) * (D / 2) + kv4_k_word(D, pg, h * JB, q4) * 4;
+                lds_words<JB>(ta, kp);
+                lds_words<JB>(tb, kp + 8 * (D / 2));
 #pragma unroll
                 for (int i = 0; i < JB; i++) { wa[h * JB + i] = ta[i]; wb[h * JB + i] = tb[i]; }
             }
-            uint32_t sa[NG / 2], sb[NG / 2];
-            lds_words<NG / 2>(sa, st + C::KS + ra * NG * 2);
-            lds_words<NG / 2>(sb, st + C::KS + (ra + 8) * NG * 2);
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) z[nt][sub][e] = 0.f;
+            float sa[NG], sb[NG];
+            lds_floats<NG>(sa, (const float *)(own + C::KF) + (at + pg) * NG);
+            lds_floats<NG>(sb, (const float *)(own + C::KF) + (at + pg + 8) * NG);
+            pw[0] = *(const float2 *)(own + C::PW + (at + pg) * 8);
+            pw[1] = *(const float2 *)(own + C::PW + (at + pg + 8) * 8);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
-                const uint32_t a0 = wa[j] & 0x000f000fu, a1 = wb[j] & 0x000f000fu;
-                const uint32_t a2 = wa[j] & 0x00f000f0u, a3 = wb[j] & 0x00f000f0u;
                 const uint32_t xa = wa[j] >> 8, xb = wb[j] >> 8;
-                const uint32_t e0 = xa & 0x000f000fu, e1 = xb & 0x000f000fu;
-                const uint32_t e2 = xa & 0x00f000f0u, e3 = xb & 0x00f000f0u;
-                const float fa = (j & 1) ? bf16hi(sa[j / 2]) : bf16lo(sa[j / 2]);
-                const float fb = (j & 1) ? bf16hi(sb[j / 2]) : bf16lo(sb[j / 2]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    float c[4] = {cinit[nt][j][0], cinit[nt][j][1], cinit[nt][j][0], cinit[nt][j][1]};
-                    mma_f16(c, a0, a1, a2, a3, Q[nt][j][0], Q[nt][j][1]);
-                    mma_f16(c, e0, e1, e2, e3, Q[nt][j][2], Q[nt][j][3]);
-                    z[nt][sub][0] = fmaf(fa, c[0], z[nt][sub][0]);
-                    z[nt][sub][1] = fmaf(fa, c[1], z[nt][sub][1]);
-                    z[nt][sub][2] = fmaf(fb, c[2], z[nt][sub][2]);
-                    z[nt][sub][3] = fmaf(fb, c[3], z[nt][sub][3]);
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(c, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u,
+                            Q[nt][j][0], Q[nt][j][1]);
+                    mma_f16(c, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, Q[nt][j][2],
+                            Q[nt][j][3]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = c[i] + cinit[nt][j][i & 1], s = i < 2 ? sa[j] : sb[j];
+                        z[nt][i] = j ? fmaf(s, x, z[nt][i]) : s * x;
+                    }
                 }
             }
         }
-        // ---- running maximum: raised only when a score passes it by more than
-        // 2^8, which keeps every weight and sum well inside fp32 and BF16
+        // ---- running maximum of z + E, so of what a position adds to the output:
+        // its weight times 2^E, and times a scale below 2, then fits f16 with the
+        // largest at 2^5 to 2^13 whatever the scales' range (what is below 2^-37 of
+        // the largest adds nothing).  It is raised only when a score passes it by
+        // more than 2^13.
+        uint32_t hide = 0;             // bit nt * 4 + i (MASKED)
         bool over = false;
-        uint32_t hide = 0;             // bit nt * SUB * 4 + sub * 4 + e (MASKED)
+        float high[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            int tail[2] = {0, 0};      // where each column's incomplete pool begins
+            int tail[2] = {0, 0};      // where a column's incomplete pool begins
             const uint8_t *srow[2] = {nullptr, nullptr};
-            if (MASKED && a.sel) {
+            if (SEL) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     tail[u] = lim[nt][u] > 0 ? lim[nt][u] - lim[nt][u] % a.pool : 0;
@@ -373,34 +419,36 @@ __global__ void __launch_bounds__(kv4::THREADS, NT == 1 ? 3 : 2) k_kv4_attn(cons
                 }
             }
 #pragma unroll
-            for (int sub = 0; sub < SUB; sub++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float v = z[nt][sub][e] * fac[nt][e & 1];
-                    if (MASKED) {
-                        const int j = pos0 + sub * 16 + (e >> 1) * 8 + pg;
-                        bool see = j < lim[nt][e & 1];
-                        if (a.sel && see && j < tail[e & 1]) {
-                            const long pl = (long)(((uint64_t)(uint32_t)j * a.pool_magic) >> 36);
-                            see = pl < a.sel_stride && srow[e & 1][pl] != 0;
-                        }
-                        if (!see) { v = NEG_INF; hide |= 1u << ((nt * SUB + sub) * 4 + e); }
+            for (int i = 0; i < 4; i++) {
+                float v = fmaf(z[nt][i], fac[nt][i & 1], pw[i >> 1].x);
+                if (MASKED) {
+                    const int o = (i >> 1) * 8 + pg;
+                    const int j = SEL ? (o < n && names[o] != 0xffff ? pos0 + names[o] : 0x7fffffff) : pos0 + o;
+                    bool see = j < lim[nt][i & 1];
+                    if (SEL && see && j < tail[i & 1]) {
+                        const long pl = (long)(((uint64_t)(uint32_t)j * a.pool_magic) >> 36);
+                        see = pl < a.sel_stride && srow[i & 1][pl] != 0;
                     }
-                    z[nt][sub][e] = v;
-                    over |= v > m[nt][e & 1] + 8.0f;
+                    if (!see) { v = NEG_INF; hide |= 1u << (nt * 4 + i); }
                 }
+                z[nt][i] = v;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                high[nt][u] = fmaxf(z[nt][u], z[nt][u + 2]);
+                over |= high[nt][u] > m[nt][u] + 13.0f;
+            }
         }
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    float x = m[nt][u];
-#pragma unroll
-                    for (int sub = 0; sub < SUB; sub++) x = fmaxf(x, fmaxf(z[nt][sub][u], z[nt][sub][u + 2]));
+                    float x = high[nt][u];
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                    if (!(x > m[nt][u] + 8.0f)) continue;          // each column by its own scores alone
+                    if (!(x > m[nt][u] + 13.0f)) continue;         // each column by its own scores alone
+                    x -= 5.0f;
                     const float down = m[nt][u] == NEG_INF ? 0.f : ex2(m[nt][u] - x);
                     m[nt][u] = x;
                     l[nt][u] *= down;
@@ -408,75 +456,251 @@ __global__ void __launch_bounds__(kv4::THREADS, NT == 1 ? 3 : 2) k_kv4_attn(cons
                     for (int i = 0; i < D / 16; i++) { O[nt][i][u] *= down; O[nt][i][u + 2] *= down; }
                 }
         }
-        // ---- weights and output
+        // ---- weights (times 2^E), brought to the order of the output's operand:
+        // column g, positions 0, 1 and 2, 3 of the lane
+        uint32_t b0[NT], b1[NT], k0[NT], k1[NT];
 #pragma unroll
-        for (int sub = 0; sub < SUB; sub++) {
-            uint32_t b0[NT], b1[NT], k0[NT], k1[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float p[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float mm = m[nt][e & 1];
-                    p[e] = ex2(z[nt][sub][e] - (MASKED && mm == NEG_INF ? 0.f : mm));
-                    // a hidden position's weight is -0: it adds nothing to the sum, and its
-                    // sign marks it below, where a NaN scale must not reach the product
-                    if (MASKED && (hide >> ((nt * SUB + sub) * 4 + e) & 1)) p[e] = -0.0f;
-                    l[nt][e & 1] += p[e];
-                }
-                b0[nt] = movmatrix(pack_bf16(p[0], p[1]));
-                b1[nt] = movmatrix(pack_bf16(p[2], p[3]));
-                if (MASKED) {
-                    k0[nt] = ~sign_bf16x2(b0[nt]);
-                    k1[nt] = ~sign_bf16x2(b1[nt]);
-                }
-            }
-            // the four positions of this lane: 0, 1 and 2, 3 are the two pairs of a fragment
-            const int r[4] = {sub * 16 + q4, sub * 16 + vp1, sub * 16 + 8 + q4, sub * 16 + 8 + vp1};
-            uint32_t w[4][D / 64], s[4][NG / 2];
+        for (int nt = 0; nt < NT; nt++) {
+            float p[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                lds_words<D / 64>(w[i], st + C::VC + r[i] * (D / 2) + kv4_v_word(D, (i & 1) ? vp1 : q4, g, 0) * 4);
-                lds_words<NG / 2>(s[i], st + C::VS + r[i] * NG * 2);
+                const float mm = m[nt][i & 1];
+                p[i] = ex2(z[nt][i] - (MASKED && mm == NEG_INF ? 0.f : mm));
+                // a hidden position's weight is -0: it adds nothing to the sum, and its
+                // sign marks it below, where a NaN scale must not reach the product
+                if (MASKED && (hide >> (nt * 4 + i) & 1)) p[i] = -0.0f;
+                l[nt][i & 1] = fmaf(p[i], pw[i >> 1].y, l[nt][i & 1]);
             }
+            b0[nt] = movmatrix(pack_f16(p[0], p[1]));
+            b1[nt] = movmatrix(pack_f16(p[2], p[3]));
+            if (MASKED) {
+                k0[nt] = ~sign_x2(b0[nt]);
+                k1[nt] = ~sign_x2(b1[nt]);
+            }
+        }
+        // ---- output
+        uint32_t w[4][D / 64], va[NG], vb[NG];
 #pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const uint32_t pick = (j & 1) ? 0x7632 : 0x5410;
-                const uint32_t s01 = __byte_perm(s[0][j / 2], s[1][j / 2], pick);
-                const uint32_t s23 = __byte_perm(s[2][j / 2], s[3][j / 2], pick);
-                const uint32_t x = __byte_perm(w[0][j / 2], w[1][j / 2], pick);
-                const uint32_t y = __byte_perm(w[2][j / 2], w[3][j / 2], pick);
-                const uint32_t x0 = code_bf16x2(x), x1 = code_bf16x2(x >> 4), x2 = code_bf16x2(x >> 8),
-                               x3 = code_bf16x2(x >> 12);
-                const uint32_t y0 = code_bf16x2(y), y1 = code_bf16x2(y >> 4), y2 = code_bf16x2(y >> 8),
-                               y3 = code_bf16x2(y >> 12);
+        for (int i = 0; i < 4; i++)
+            lds_words<D / 64>(w[i], st + C::VC + (at + (i >> 1) * 8 + ((i & 1) ? vp1 : q4)) * (D / 2) +
+                                        kv4_v_word(D, (i & 1) ? vp1 : q4, g, 0) * 4);
+        lds_pairs<NG>(va, (const uint32_t *)(own + C::VH) + ((at >> 3) * 4 + q4) * NG);
+        lds_pairs<NG>(vb, (const uint32_t *)(own + C::VH) + ((at >> 3) * 4 + 4 + q4) * NG);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    uint32_t w0 = mul_bf16x2(b0[nt], s01), w1 = mul_bf16x2(b1[nt], s23);
-                    if (MASKED) { w0 &= k0[nt]; w1 &= k1[nt]; }
-                    mma_bf16(O[nt][2 * j], x0, x1, y0, y1, w0, w1);
-                    mma_bf16(O[nt][2 * j + 1], x2, x3, y2, y3, w0, w1);
-                }
+        for (int j = 0; j < NG; j++) {
+            const uint32_t pick = (j & 1) ? 0x7632 : 0x5410;
+            const uint32_t x = __byte_perm(w[0][j / 2], w[1][j / 2], pick);
+            const uint32_t y = __byte_perm(w[2][j / 2], w[3][j / 2], pick);
+            const uint32_t x0 = code_lo(x, cc), x1 = code_hi(x, cc), x2 = code_lo(x >> 8, cc), x3 = code_hi(x >> 8, cc);
+            const uint32_t y0 = code_lo(y, cc), y1 = code_hi(y, cc), y2 = code_lo(y >> 8, cc), y3 = code_hi(y >> 8, cc);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                uint32_t w0 = mul_f16x2(b0[nt], va[j]), w1 = mul_f16x2(b1[nt], vb[j]);
+                if (MASKED) { w0 &= k0[nt]; w1 &= k1[nt]; }
+                mma_f16(O[nt][2 * j], x0, x1, y0, y1, w0, w1);
+                mma_f16(O[nt][2 * j + 1], x2, x3, y2, y3, w0, w1);
             }
         }
     };
 
-    // ---- the stream
-    static_assert(kv4::STAGES == 2, "the units in flight are held in two variables");
-    Unit now = load(0), next = load(1);
-    for (int i = 0; i < mine; i++) {
-        const bool got = mbar_wait(&full[warp][i % 2], (i / 2) & 1, ab, &g_kv4a_err, (int)ATTN_ERR_WAIT);
-        if (!__all_sync(0xffffffffu, got)) break;
-        const uint8_t *st = stages + (i % 2) * C::STAGE;
-        const int pos0 = p0 + now.u * U;
-        if (now.page >= 0) {
-            if (!a.sel && pos0 + U <= lim0) process(st, pos0, std::false_type{});
-            else process(st, pos0, std::true_type{});
+    // ---- the stream: this warp's units warp, warp + WARPS, ... of the piece, or
+    // of one list of selected positions after the other
+    int done = p0;
+    do {
+        int base = p0, filled = p1 > p0 ? p1 - p0 : 0;     // positions, the first of them (SEL: of the list)
+        if constexpr (SEL) {
+            // list the positions from `done` on that a row keeps, as many as the
+            // list holds: a thread looks at one pool
+            __syncthreads();
+            const int t0 = lim0 - lim_row0, t1 = lim1 - lim_row0;          // rows of the block
+            const int span = min(p1, done + kv4::LIST_SPAN);
+            base = done;
+            filled = 0;
+            // pools looked at together: one at least (a pool has at most 128
+            // positions, the list room for 2048), so `done` advances each time
+            const int round = min(kv4::THREADS, C::LIST / a.pool);
+            while (done < span && filled + round * a.pool <= C::LIST) {
+                const int pl = done / a.pool + (int)threadIdx.x;
+                const int b = max(pl * a.pool, done), e = min((pl + 1) * a.pool, span);
+                bool any = false;
+                if ((int)threadIdx.x < round && b < e)
+                    for (int t = t0; t <= t1; t++) {
+                        const int lim = lim_row0 + t;
+                        if (lim <= b) continue;
+                        any |= b >= lim - lim % a.pool ||
+                               (pl < a.sel_stride && a.sel[(long)(sq.row0 + t) * a.sel_stride + pl] != 0);
+                    }
+                const int cnt = any ? e - b : 0;
+                int incl = cnt;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, incl, off);
+                    if (lane >= off) incl += o;
+                }
+                if (lane == 31) wcount[warp] = incl;
+                __syncthreads();
+                int at = filled + incl - cnt;
+                for (int w = 0; w < warp; w++) at += wcount[w];
+                for (int i = 0; i < cnt; i++) list[at + i] = (uint16_t)(b + i - base);
+                for (int w = 0; w < kv4::WARPS; w++) filled += wcount[w];
+                done = min(span, (done / a.pool + round) * a.pool);
+                __syncthreads();
+            }
         }
-        __syncwarp();
-        now = next;
-        next = load(i + 2);
-    }
+        const int units = (filled + U - 1) / U;
+        const int mine = units > warp ? (units - warp + kv4::WARPS - 1) / kv4::WARPS : 0;
+        int my_page = -1;                  // lane i: page of the i-th of 32 units
+        unsigned there = 0;                // bit s: stage s holds a unit (not one of a page out of range)
+        auto load = [&](int i, int s) {    // unit i of this warp into stage s (whole warp)
+            if (i < mine) {
+                const int u = warp + i * kv4::WARPS;
+                uint8_t *dst = stages + s * C::STAGE;
+                constexpr int CH = D / 32;                 // 16-byte pieces of a row of codes
+                if constexpr (!SEL) {
+                    if ((i & 31) == 0) {
+                        my_page = -1;
+                        if (i + lane < mine) {
+                            const int page = table[(p0 + (u + lane * kv4::WARPS) * U) / KV4_PAGE];
+                            if (kv4_page_ok(page, a.v.num_pages)) my_page = page;
+                            else atomicExch(&g_kv4a_err, (int)ATTN_ERR_PAGE);
+                        }
+                    }
+                    const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
+                    there = (there & ~(1u << s)) | ((page >= 0 ? 1u : 0u) << s);
+                    if (page >= 0) {
+                        const int h = u % UPP;             // pieces begin at a page
+                        const uint8_t *src = a.v.pages + kv4_block_at(page, head, a.v.heads, D);
+                        const uint8_t *kc = src + h * (U * D / 2) + lane * 16;
+#pragma unroll
+                        for (int k = 0; k < U * CH / 32; k++) {
+                            cp_async16(dst + C::KC + lane * 16 + k * 512, kc + k * 512);
+                            cp_async16(dst + C::VC + lane * 16 + k * 512, kc + kv4_v_codes(D) + k * 512);
+                        }
+                        // scales: 16 pieces of the keys', 16 of the values'
+                        cp_async16(dst + C::KS + lane * 16, src + (lane < 16 ? kv4_k_scales(D) : kv4_v_scales(D)) +
+                                                                h * 256 + (lane & 15) * 16);
+                        static_assert(U * NG * 2 == 256 && C::VS == C::KS + 256, "scales of a unit");
+                    }
+                } else {
+                    constexpr int RPL = (U + 31) / 32;     // rows a lane finds
+                    const int u0 = u * U;
+                    const uint8_t *src[RPL];
+                    int off[RPL];
+#pragma unroll
+                    for (int e = 0; e < RPL; e++) {
+                        const int r = e * 32 + lane;
+                        src[e] = nullptr;
+                        off[e] = 0;
+                        if (r < U && u0 + r < filled) {
+                            const int j = base + list[u0 + r], page = table[j / KV4_PAGE];
+                            off[e] = j & (KV4_PAGE - 1);
+                            if (kv4_page_ok(page, a.v.num_pages)) src[e] = a.v.pages + kv4_block_at(page, head, a.v.heads, D);
+                            else {
+                                atomicExch(&g_kv4a_err, (int)ATTN_ERR_PAGE);
+                                list[u0 + r] = 0xffff;     // unseen
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < U * CH; k += 32) {
+                        const int row = (k + lane) / CH, c = (k + lane) % CH, e = (k / CH) / 32;
+                        const uint8_t *sp = (const uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)src[e], row & 31);
+                        const int o = __shfl_sync(0xffffffffu, off[e], row & 31);
+                        // the row moves from place o of its page to place `row`
+                        // of the stage, and its pieces as the layout has them there
+                        const int kx = D == 256 ? (((o ^ row) >> 2) & 1) << 2 : 0;
+                        const int vx = D == 256 ? ((o ^ row) & 3) << 1 : D == 128 ? (((o ^ row) >> 1) & 1) << 1 : 0;
+                        if (sp) {
+                            cp_async16(dst + C::KC + row * (D / 2) + (c ^ kx) * 16, sp + o * (D / 2) + c * 16);
+                            cp_async16(dst + C::VC + row * (D / 2) + (c ^ vx) * 16,
+                                       sp + kv4_v_codes(D) + o * (D / 2) + c * 16);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < RPL; e++) {
+                        const int r = e * 32 + lane;
+                        if (src[e]) {
+                            cp_async_n<NG * 2>(dst + C::KS + r * NG * 2, src[e] + kv4_k_scales(D) + off[e] * NG * 2);
+                            cp_async_n<NG * 2>(dst + C::VS + r * NG * 2, src[e] + kv4_v_scales(D) + off[e] * NG * 2);
+                        }
+                    }
+                    there |= 1u << s;
+                }
+            }
+            cp_async_commit();
+        };
+        for (int s = 0; s < kv4::STAGES; s++) load(s, s);
+        if (!SEL || base == p0) {      // once a piece, while its first units are on their way
+            // ---- the query's fragments: column g of each n tile, dims in the order
+            // in which a lane meets the key codes (dim 8 q4 + i of a group is code i
+            // of its word)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    const uint32_t w[4] = {raw[nt][j].x, raw[nt][j].y, raw[nt][j].z, raw[nt][j].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // a power of two that brings the largest magnitude to [2^14, 2^15): f16
+                // holds every BF16 within 2^-24 of it exactly, smaller ones to 2^-35 of it
+                const int e = top ? max((int)(top >> 7) - 127, -100) : 0;
+                const float up = __int_as_float((127 + 14 - e) << 23);
+                float f = a.zscale * __int_as_float((127 + e - 14) << 23) * 16777216.0f;
+                if (top >= 0x7f80u) f = __int_as_float(0x7fc00000);    // a NaN or an infinity: the row is NaN
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    const float x[8] = {bf16lo(raw[nt][j].x), bf16hi(raw[nt][j].x), bf16lo(raw[nt][j].y), bf16hi(raw[nt][j].y),
+                                        bf16lo(raw[nt][j].z), bf16hi(raw[nt][j].z), bf16lo(raw[nt][j].w), bf16hi(raw[nt][j].w)};
+                    float qs = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // codes in the high nibbles stand 16 times higher
+                        const float down = (i & 1) ? up * 0.0625f : up;
+                        const uint32_t h = pack_f16(x[i] * down, x[i + 4] * down);
+                        Q[nt][j][i] = h;
+                        const float2 back = __half22float2(*(const __half2 *)&h);
+                        qs += (back.x + back.y) * ((i & 1) ? 16.0f : 1.0f);
+                    }
+                    qs += __shfl_xor_sync(0xffffffffu, qs, 1);
+                    qs += __shfl_xor_sync(0xffffffffu, qs, 2);
+                    qs *= -8.0f / 16777216.0f;                               // the codes' offset
+                cinit[nt][j][0] = __shfl_sync(0xffffffffu, qs, 8 * q4);
+                cinit[nt][j][1] = __shfl_sync(0xffffffffu, qs, 8 * q4 + 4);
+                }
+                // what follows goes by the columns whose scores this lane holds
+            fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * q4);
+            fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * q4 + 4);
+#pragma unroll
+            for (int u = 0; u < 2; u++) lim[nt][u] = lim_row0 + row_of(a, min(c0 + nt * 8 + 2 * q4 + u, cols - 1));
+            }
+        }
+        int s = 0;
+        for (int i = 0; i < mine; i++) {
+            cp_async_wait<kv4::STAGES - 1>();
+            __syncwarp();
+            if (there >> s & 1) {
+                const uint8_t *st = stages + s * C::STAGE;
+                const int u0 = (warp + i * kv4::WARPS) * U;
+                prepare(st);
+                if (!SEL && p0 + u0 + U <= lim0) {
+#pragma unroll 1
+                    for (int at = 0; at < U; at += 16) process(st, at, p0 + u0 + at, nullptr, 0, std::false_type{});
+                } else {
+#pragma unroll 1
+                    for (int at = 0; at < U && u0 + at < filled; at += 16)
+                        process(st, at, SEL ? base : p0 + u0 + at, list + u0 + at, filled - u0 - at, std::true_type{});
+                }
+            }
+            __syncwarp();
+            load(i + kv4::STAGES, s);
+            s = s == kv4::STAGES - 1 ? 0 : s + 1;
+        }
+        cp_async_wait<0>();
+    } while (SEL && done < p1);
 
     // ---- join the warps (the stages are free once every warp is here)
 #pragma unroll
@@ -491,21 +715,22 @@ __global__ void __launch_bounds__(kv4::THREADS, NT == 1 ? 3 : 2) k_kv4_attn(cons
             }
         }
     __syncthreads();
-    float *jo = (float *)kv4_dyn;     // [WARPS][COLS][D]
+    constexpr int JD = D + 4;         // rows a bank group apart
+    float *jo = (float *)kv4_dyn;     // [WARPS][COLS][JD]
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            float *row = jo + ((size_t)warp * COLS + nt * 8 + 2 * q4 + u) * D;
+            float *row = jo + (warp * COLS + nt * 8 + 2 * q4 + u) * JD;
 #pragma unroll
             for (int j = 0; j < NG; j++)
                 *(float4 *)(row + 32 * j + 4 * g) = make_float4(O[nt][2 * j][u], O[nt][2 * j][u + 2],
                                                                O[nt][2 * j + 1][u], O[nt][2 * j + 1][u + 2]);
         }
     __syncthreads();
-    const bool last = a.nchunk == 1;
-    float *part = a.part + (((size_t)seq * gridDim.y + blockIdx.y) * a.nchunk + chunk) * (size_t)(COLS * (D + 2));
-    for (int i = threadIdx.x; i < COLS * (D / 4); i += kv4::THREADS) {
+    const bool last = starts && ends;
+    float *part = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (size_t)(COLS * (D + 2));
+    for (int i = threadIdx.x; i < (cend - c0) * (D / 4); i += kv4::THREADS) {
         const int c = i / (D / 4), d = (i % (D / 4)) * 4;
         float mx = NEG_INF;
 #pragma unroll
@@ -516,73 +741,83 @@ __global__ void __launch_bounds__(kv4::THREADS, NT == 1 ? 3 : 2) k_kv4_attn(cons
         for (int w = 0; w < kv4::WARPS; w++) {
             if (join_m[w][c] == NEG_INF && join_l[w][c] == 0.f) continue;
             const float k = ex2(join_m[w][c] - mx);
-            const float4 x = *(const float4 *)(jo + ((size_t)w * COLS + c) * D + d);
+            const float4 x = *(const float4 *)(jo + (w * COLS + c) * JD + d);
             sum += join_l[w][c] * k;
             o.x += x.x * k; o.y += x.y * k; o.z += x.z * k; o.w += x.w * k;
         }
         if (!last) {
             *(float4 *)(part + 2 * COLS + c * D + d) = o;
             if (d == 0) { part[c] = mx; part[COLS + c] = sum; }
-        } else if (c0 + c < cend) {
+        } else {
             const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-            uint16_t *op = a.out.p + (long)(sq.row0 + (c0 + c) / a.group) * a.out.rs +
-                           (long)(head * a.group + (c0 + c) % a.group) * a.out.hs + d;
+            const int t = row_of(a, c0 + c);
+            uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs +
+                           (long)(head * a.group + c0 + c - t * a.group) * a.out.hs + d;
             *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
         }
     }
+    __syncthreads();        // the stages are the next piece's
+    x = piece_e;
+    }
 }
 
-// Joins the chunks of one column: weights 2^(m_c - max m), in chunk order.
+// Joins the pieces of one column of a segment that was cut: weights
+// 2^(m_c - max m), in the order of the runs.
 template <int D>
 __global__ void __launch_bounds__(128) k_kv4_join(const Kv4AttnArgs a, int cols_block) {
-    constexpr int L = D / 4, P = 128 / L;      // lanes over the dims, parts over the chunks
-    extern __shared__ float kj_dyn[];          // [nchunk] weights, then [P][D] sums
-    __shared__ float total;
+    constexpr int L = D / 4, P = 128 / L;      // lanes over the dims, parts over the pieces
+    extern __shared__ float kj_dyn[];          // weights of the pieces, then [P][D] sums
+    __shared__ float total_s;
     const int seq = blockIdx.z, head = blockIdx.y, c = blockIdx.x;
-    const Kv4Seq sq = kv4_seq(a.v.cu[seq], a.v.cu[seq + 1], a.v.len[seq], a.v.rows, a.v.max_rows, a.v.max_len);
-    const int cols = sq.n * a.group;
-    if (c >= cols) return;
+    const Kv4Work wk = kv4_work(a, seq, cols_block);
+    const Kv4Seq sq = wk.sq;
+    pdl_wait();                                // the partial results and the plan
+    if (c >= sq.n * a.group) return;
     const int cb = c / cols_block, cc = c % cols_block;
-    const int lim1 = sq.len - sq.n + 1 + (min((cb + 1) * cols_block, cols) - 1) / a.group;
-    const int n = lim1 > 0 ? min((lim1 + a.chunk_pos - 1) / a.chunk_pos, a.nchunk) : 0;
+    const long runs = a.plan[0], total = a.plan[1];
+    const long b = a.plan[2 + seq] + ((long)head * wk.ncb + cb) * wk.pages, e = b + wk.pages;
+    const long i0 = ((b + 1) * runs - 1) / total, i1 = (e * runs - 1) / total;   // runs of the first and the last page
+    if (i0 == i1) return;                      // written by its only run
+    const int n = (int)(i1 - i0) + 1;
     const size_t stride = (size_t)cols_block * (D + 2);
-    const float *base = a.part + (((size_t)seq * a.v.heads + head) * a.ncb + cb) * a.nchunk * stride;
-    float *sums = kj_dyn + (a.nchunk + 3) / 4 * 4;
+    auto piece = [&](int i) { return a.part + ((size_t)(i0 + i) * 2 + (i == 0 ? 1 : 0)) * stride; };
+    float *sums = kj_dyn + KJ_RUNS;
     if (threadIdx.x < 32) {
         float mx = kv4::NEG_INF;
-        for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, base[i * stride + cc]);
+        for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, piece(i)[cc]);
 #pragma unroll
         for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         float sum = 0.f;
         for (int i = threadIdx.x; i < n; i += 32) {
-            const float mi = base[i * stride + cc], li = base[i * stride + cols_block + cc];
+            const float mi = piece(i)[cc], li = piece(i)[cols_block + cc];
             const float k = mi == kv4::NEG_INF && li == 0.f ? 0.f : ex2(mi - mx);
             kj_dyn[i] = k;
             sum += li * k;
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (threadIdx.x == 0) total = sum;
+        if (threadIdx.x == 0) total_s = sum;
     }
     __syncthreads();
     const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int i = part; i < n; i += P) {
         const float k = kj_dyn[i];
-        if (k == 0.f) continue;                // a chunk that saw nothing
-        const float4 x = *(const float4 *)(base + i * stride + 2 * cols_block + cc * D + d);
-        o.x += x.x * k; o.y += x.y * k; o.z += x.z * k; o.w += x.w * k;
+        const float4 y = *(const float4 *)(piece(i) + 2 * cols_block + cc * D + d);
+        if (k != 0.f) { o.x += y.x * k; o.y += y.y * k; o.z += y.z * k; o.w += y.w * k; }   // 0: it saw nothing
     }
     *(float4 *)(sums + part * D + d) = o;
     __syncthreads();
     if (part) return;
 #pragma unroll
     for (int i = 1; i < P; i++) {
-        const float4 x = *(const float4 *)(sums + i * D + d);
-        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        const float4 y = *(const float4 *)(sums + i * D + d);
+        o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
     }
-    const float inv = total == 0.f ? 0.f : 1.0f / total;
-    uint16_t *op = a.out.p + (long)(sq.row0 + c / a.group) * a.out.rs + (long)(head * a.group + c % a.group) * a.out.hs + d;
+    const float inv = total_s == 0.f ? 0.f : 1.0f / total_s;
+    const int t = row_of(a, c);
+    uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs + (long)(head * a.group + c - t * a.group) * a.out.hs + d;
     *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
@@ -591,26 +826,23 @@ using namespace apus;
 
 namespace {
 
-// How a batch is cut: columns of a block and positions of a chunk.
-constexpr long MAX_CHUNK = 1024;              // pages: bounds the list of units in shared memory
-constexpr long MAX_POS = 1l << 28;            // bounds the joining kernel's weights
-struct Kv4Plan { int nt, ncb, chunk_pages, nchunk; size_t bytes; };
+// How a batch is cut: columns of a block, CTAs, whether segments stay whole.
+constexpr long MAX_POS = 1l << 28;
+constexpr long WHOLE_PAGES = 8, MIN_PAGES = 2;
+struct Kv4Plan { int nt, grid, whole; size_t plan_bytes, bytes; };
 
 Kv4Plan kv4_plan(const Kv4View &v, size_t q_heads) {
     Kv4Plan p;
-    const long group = (long)q_heads / v.heads, cols = group * v.max_rows;
+    const long cols = (long)q_heads / v.heads * v.max_rows;
     p.nt = cols > 8 && v.dim <= 128 ? 2 : 1;
-    p.ncb = (int)((cols + 8 * p.nt - 1) / (8 * p.nt));
-    const long pages = (v.max_len + KV4_PAGE - 1) / KV4_PAGE, base = (long)v.nseq * v.heads * p.ncb;
-    const long slots = 148 * 3 * 4;
-    long want = (base * pages + slots - 1) / slots;          // pages of a chunk for that many CTAs
-    if (want < 8) want = 8;                                  // two pages a warp at least
-    if (want < (pages + 255) / 256) want = (pages + 255) / 256;
-    if (want > MAX_CHUNK) want = MAX_CHUNK;
-    if (want > pages) want = pages > 0 ? pages : 1;
-    p.chunk_pages = (int)want;
-    p.nchunk = pages > 0 ? (int)((pages + want - 1) / want) : 1;
-    p.bytes = p.nchunk > 1 ? (size_t)base * p.nchunk * (8 * p.nt) * (v.dim + 2) * sizeof(float) : 0;
+    const long pages = v.max_len > KV4_PAGE ? (v.max_len + KV4_PAGE - 1) / KV4_PAGE : 1;
+    const long segs = (long)v.nseq * v.heads * ((cols + 8 * p.nt - 1) / (8 * p.nt));
+    p.whole = pages <= WHOLE_PAGES;
+    const long most = p.whole ? segs : (segs * pages + MIN_PAGES - 1) / MIN_PAGES, slots = 148 * kv4::resident(p.nt);
+    p.grid = (int)(most < slots ? most : slots);
+    p.plan_bytes = ((size_t)v.nseq + 2) * sizeof(long);
+    p.plan_bytes = (p.plan_bytes + 15) / 16 * 16;
+    p.bytes = p.whole ? 0 : p.plan_bytes + (size_t)p.grid * 2 * (8 * p.nt) * (v.dim + 2) * sizeof(float);
     return p;
 }
 
@@ -634,17 +866,29 @@ int kv4_attn_args(const char *what, const ApusKv4Cache *c, const ApusKv4Batch *b
     return 0;
 }
 
-template <int D, int NT>
-int kv4_attn_launch(const Kv4AttnArgs &a, cudaStream_t st) {
+template <int D, int NT, bool SEL>
+int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     using C = kv4::Cfg<D>;
-    const int smem = C::SMEM + (a.sel ? (a.chunk_pos / C::U) * 2 : 0);
-    if (gcuda_smem_limit_once((const void *)k_kv4_attn<D, NT>, smem)) return -1;
-    k_kv4_attn<D, NT><<<dim3(a.nchunk, a.v.heads * a.ncb, a.v.nseq), kv4::THREADS, smem, st>>>(a);
+    const int smem = C::SMEM + (SEL ? C::LIST * 2 : 0);
+    if (gcuda_smem_limit_once((const void *)k_kv4_attn<D, NT, SEL>, smem)) return -1;
+    k_kv4_attn<D, NT, SEL><<<grid, kv4::THREADS, smem, st>>>(a);
     if (gcuda_check(cudaGetLastError(), "kv4_attn launch")) return -1;
-    if (a.nchunk == 1) return 0;
-    const int jsmem = ((a.nchunk + 3) / 4 * 4 + (128 / (D / 4)) * D) * 4;
-    k_kv4_join<D><<<dim3(a.group * a.v.max_rows, a.v.heads, a.v.nseq), 128, jsmem, st>>>(a, 8 * NT);
-    return gcuda_check(cudaGetLastError(), "kv4_attn join launch");
+    if (a.whole) return 0;
+    // the joining kernel starts while the first drains, and waits for it
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.group * a.v.max_rows, a.v.heads, a.v.nseq);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = (KJ_RUNS + (128 / (D / 4)) * D) * 4;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return gcuda_check(cudaLaunchKernelEx(&cfg, k_kv4_join<D>, a, 8 * NT), "kv4_attn join launch");
+}
+template <int D, int NT> int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
+    return a.sel ? kv4_attn_launch<D, NT, true>(a, grid, st) : kv4_attn_launch<D, NT, false>(a, grid, st);
 }
 
 }  // namespace
@@ -682,19 +926,20 @@ extern "C" int apus_gcuda_kv4_attn_dev(const ApusKv4Cache *cache, const ApusKv4B
     a.q = rows_view(q);
     a.out = rows_view(out);
     a.group = (int)(q->heads / cache->heads);
+    a.group_magic = (((uint64_t)1 << 40) + (uint64_t)a.group - 1) / (uint64_t)a.group;
     a.zscale = scale * 1.4426950408889634f;
     a.sel = sel;
     a.sel_stride = (long)sel_stride;
     a.pool = sel ? (int)pool : 1;
     a.pool_magic = (((uint64_t)1 << 36) + (uint64_t)a.pool - 1) / (uint64_t)a.pool;
-    a.chunk_pos = p.chunk_pages * KV4_PAGE;
-    a.nchunk = p.nchunk;
-    a.ncb = p.ncb;
-    a.part = (float *)workspace;
+    a.whole = p.whole;
+    a.min_pages = p.whole ? 1 : (int)MIN_PAGES;
+    a.plan = p.whole ? nullptr : (long *)workspace;
+    a.part = p.whole ? nullptr : (float *)((char *)workspace + p.plan_bytes);
     cudaStream_t st = (cudaStream_t)stream;
-    if (cache->dim == 64) return p.nt == 2 ? kv4_attn_launch<64, 2>(a, st) : kv4_attn_launch<64, 1>(a, st);
-    if (cache->dim == 128) return p.nt == 2 ? kv4_attn_launch<128, 2>(a, st) : kv4_attn_launch<128, 1>(a, st);
-    return kv4_attn_launch<256, 1>(a, st);
+    if (cache->dim == 64) return p.nt == 2 ? kv4_attn_launch<64, 2>(a, p.grid, st) : kv4_attn_launch<64, 1>(a, p.grid, st);
+    if (cache->dim == 128) return p.nt == 2 ? kv4_attn_launch<128, 2>(a, p.grid, st) : kv4_attn_launch<128, 1>(a, p.grid, st);
+    return kv4_attn_launch<256, 1>(a, p.grid, st);
 }
 
 int kv4_attn_error_read_and_clear(void) {

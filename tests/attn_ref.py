@@ -1,12 +1,13 @@
 """Plain 64-bit references of the operators of include/apus_attn_gcuda.h, and
 the error bounds that their tests use.
 
-A BF16 rounding is off by at most U = 2^-8 of the value."""
+A BF16 rounding is off by at most U = 2^-8 of the value, an f16 rounding by
+H = 2^-11."""
 import numpy as np
 import torch
 
 PAGE = 64
-U = 2.0 ** -8
+U, H = 2.0 ** -8, 2.0 ** -11
 
 
 def word_and_code(dim, p, d):
@@ -57,14 +58,19 @@ def held(codes, scales):
     return ((codes.double() - 8).unflatten(-1, (-1, 32)) * scales[..., None]).flatten(-2)
 
 
-def attention(q, k, v, scale, seen, extra=None):
-    """Rows q [r][heads][dim] over k, v [n][kv heads][dim] (64 bits), seen [r][n]: (out, spread, slack).
+def attention(q, k, v, scale, seen, extra=None, steps=None):
+    """Rows q [r][heads][dim] over k, v [n][kv heads][dim] (64 bits), seen [r][n]: (out, spread, slack, floor).
     spread is sum p |v| / sum p; slack bounds the relative error of a weight that fp32 sums of the scores make:
     each of the dim products (and each term of `extra`, [n][kv heads][dim]: further magnitudes that a kernel adds
-    and takes away again) takes part in at most dim + 8 additions off by 2^-22 of the running sum."""
+    and takes away again) takes part in at most dim + 8 additions off by 2^-22 of the running sum.
+    floor is what f16's least step adds where `steps`, [n][kv heads], the largest value scale of each position, is
+    given.  With 2^E <= steps < 2^(E + 1), p 2^E is held in f16 in a unit in which the largest one of the row is 2^5 at
+    least, and the scales divided by 2^E, below 2, too.  Below 2^-14 a rounding is off by 2^-25 at most, so (codes of at
+    most 7): 7 * 2 * 2^-30 max(p 2^E) a position for p 2^E, 7 * 2^-30 max(p 2^E) for its product with a scale, and
+    7 * 2^-25 p 2^E for the scale."""
     r, heads, dim = q.shape
     if not k.shape[0]:
-        return torch.zeros_like(q), torch.zeros_like(q), 0.0
+        return torch.zeros_like(q), torch.zeros_like(q), 0.0, 0.0
     group = heads // k.shape[1]
     k, v = (x.repeat_interleave(group, 1) for x in (k, v))
     hide = ~seen[:, None, :]
@@ -78,14 +84,18 @@ def attention(q, k, v, scale, seen, extra=None):
     mag = k.abs() if extra is None else k.abs() + extra.repeat_interleave(group, 1)
     size = torch.einsum("rhd,nhd->rhn", q.abs(), mag).masked_fill(hide, 0.0).amax(-1, keepdim=True)
     slack = 2 * (dim + 8) * 2.0 ** -22 * abs(scale) * size + k.shape[0] * 2.0 ** -24 + 2.0 ** -20
-    return out, spread, slack
+    floor = 0.0
+    if steps is not None:
+        held = w * steps.T.repeat_interleave(group, 0)
+        floor = 21 * k.shape[0] * 2.0 ** -30 * held.amax(-1, keepdim=True) + 7 * 2.0 ** -25 * held.sum(-1, keepdim=True)
+    return out, spread, slack, floor
 
 
-def bound(out, spread, slack, roundings):
-    """What a kernel may be off: each weight by `roundings` BF16 roundings and the scores' slack, the result by one
-    rounding (and by half a step of the smallest BF16 number)."""
-    rel = (1 + U) ** roundings * (1 + slack) - 1
-    return U * out.abs() + (1 + U) * (rel + slack) * spread + 2.0 ** -134
+def bound(out, spread, slack, floor, weight):
+    """What a kernel may be off: each weight by its roundings (`weight`, relative) and the scores' slack, the result by
+    one BF16 rounding (and by half a step of the smallest BF16 number)."""
+    rel = (1 + weight) * (1 + slack) - 1
+    return U * out.abs() + (1 + U) * ((rel + slack) * spread + floor) + 2.0 ** -134
 
 
 def assert_within(got, want, most, what=""):
