@@ -9,6 +9,12 @@ int attn_check_dim(const char *what, size_t dim) {
     return -1;
 }
 
+int attn_check_scale(const char *what, float scale) {
+    if (scale > 0.0f && scale < 1e30f) return 0;
+    gcuda_set_error("%s: scale %g (positive)", what, (double)scale);
+    return -1;
+}
+
 int attn_check_rows(const char *what, const ApusHeadRows *r, size_t dim, bool output) {
     if (!r) { gcuda_set_error("%s: no rows given", what); return -1; }
     const size_t lim = (size_t)1 << 31;

@@ -28,6 +28,7 @@ struct RowsView {
 // Argument checks (attn_check.cu); each records the reason and returns -1.
 int attn_check_rows(const char *what, const ApusHeadRows *r, size_t dim, bool output);
 int attn_check_dim(const char *what, size_t dim);
+int attn_check_scale(const char *what, float scale);
 int kv4_check(const char *what, const ApusKv4Cache *c, const ApusKv4Batch *b, size_t rows, Kv4View *out);
 static inline RowsView rows_view(const ApusHeadRows *r) {
     return RowsView{r->p, (long)r->row_stride, (long)r->head_stride};

@@ -906,7 +906,7 @@ extern "C" int apus_gcuda_kv4_attn_dev(const ApusKv4Cache *cache, const ApusKv4B
     const char *what = "kv4_attn";
     if (!q || !out) { gcuda_set_error("%s: no rows given", what); return -1; }
     Kv4AttnArgs a{};
-    if (kv4_attn_args(what, cache, batch, q->heads, q->rows, &a.v)) return -1;
+    if (kv4_attn_args(what, cache, batch, q->heads, q->rows, &a.v) || attn_check_scale(what, scale)) return -1;
     if (attn_check_rows(what, q, cache->dim, false) || attn_check_rows(what, out, cache->dim, true)) return -1;
     if (q->rows != out->rows || q->heads != out->heads) {
         gcuda_set_error("%s: %zu rows of %zu heads in, %zu of %zu out", what, q->rows, q->heads, out->rows, out->heads);

@@ -1,9 +1,40 @@
 // prompt_attn.cu — causal attention over packed sequences with grouped heads
 // (apus_gcuda_prompt_attn_dev):
 //   out_i = sum_{j <= m - n + i} p_ij v_j,  p_i = softmax_j(scale q_i . k_j)
-// for row i of n queries over m keys of one sequence.
+// for row i of n queries over m keys of one sequence, in one pass over the keys
+// with a running maximum and sum.
+//
+// Both products run on tcgen05: a CTA takes NQ tiles of 128 query rows of one
+// head and walks the keys in tiles of 128,
+//   S (TMEM, fp32) = Q (shared) . K^T (shared),   O (TMEM, fp32) += P (TMEM) . V (shared),
+// with P = 2^(scale log2(e) (S - maximum)) in BF16 written over S.  K and V come as
+// tensor copies (128-byte swizzle) into a ring; V is read as it lies, rows of
+// keys with the dims contiguous.
+//
+// Bound: at dim 256 the products (2048 tensor cycles a tile of 128 x 128), at
+// dim 128 products and exponentials alike (1024 tensor cycles; 16384
+// exponentials at 16 a cycle), at dim 64 the exponentials.
+// So two query tiles share an SM up to dim 128: one tile's softmax runs under
+// the other's products.  At dim 256 the accumulator of one tile fills half of
+// TMEM and two S tiles the other half: the next tile's S is computed under this
+// tile's softmax.
+//
+// Roles: warp 0 copies, warp 1 issues the products, warps 2-3 look after V tiles
+// with keys that some row must not see, warps 4.. are one softmax group of 128
+// threads (a row each) a query tile.  The maximum is raised, and O rescaled, only
+// when a score passes it by more than 2^8, so almost never.
+//
+// A hidden key's weight is 0, but 0 times a NaN or an infinity in its value would
+// reach the row through the product.  So in tiles with hidden keys such values
+// (and all rows behind the sequence) are set to 0 in shared memory before the
+// product reads them; the first key with a NaN, a +inf and a -inf is kept for each
+// dim, and the rows that see it get it added at the end.
+#include <type_traits>
+
 #include "attn_dev.h"
 #include "common.cuh"
+#include "pipe.cuh"
+#include "tc.cuh"
 
 namespace apus {
 
@@ -14,7 +45,7 @@ struct PromptArgs {
     int nseq, rows_q, rows_k, max_rows;
     RowsView q, k, v, out;
     int heads, group;          // query heads, query heads of a key head
-    float zscale;              // scale * log2(e)
+    float zscale;              // scale * log2(e), positive
 };
 
 // A sequence's ranges; one that is out of bounds is empty.
@@ -26,62 +57,476 @@ APUS_DEV PromptSeq prompt_seq(const PromptArgs &a, int s, bool report) {
     return PromptSeq{q.row0, q.n, k.row0, k.n};
 }
 
-// One warp a query row and head, the keys one after another; a lane holds
-// D / 32 neighbouring dims.
+namespace pa {
+constexpr int BM = 128, BN = 128;               // query rows of a tile, keys of a tile
+constexpr int PANEL = 128 * 128;                // bytes of 128 rows of 64 dims
+template <int D> struct Cfg {
+    static constexpr int NQ = D == 256 ? 1 : 2;             // query tiles of a CTA
+    static constexpr int THREADS = 128 + 128 * NQ;
+    static constexpr int SPAN = D == 256 ? 128 : D;         // dims of a ring stage
+    static constexpr int PARTS = D / SPAN;                  // stages of a K or V tile
+    static constexpr int STAGE = SPAN / 64 * PANEL;
+    static constexpr int QTILE = D / 64 * PANEL;
+    static constexpr int NST = D == 256 ? 5 : D == 128 ? 4 : 8;
+    static constexpr int SMEM = NQ * QTILE + NST * STAGE + 1024;
+    static constexpr int ROWS = NQ * BM;
+    static constexpr int O_COL = 256;                       // TMEM: S tiles at 0 and 128, O from 256
+    // D f32, A and B BF16, N >> 3 at bit 17, M >> 4 at bit 24; V has its dims
+    // (N) contiguous: bit 16
+    static constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
+                                        ((uint32_t)(BM >> 4) << 24);
+    static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) |
+                                        ((uint32_t)(SPAN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+};
+constexpr float RAISE = 8.0f;
+}  // namespace pa
+
+APUS_DEV float pa_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+APUS_DEV uint32_t pa_pack(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
 template <int D>
-__global__ void __launch_bounds__(128) k_prompt_rows(const PromptArgs a) {
-    constexpr int E = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.y;
-    const long row = (long)blockIdx.x * 4 + warp;
-    if (row >= a.rows_q) return;
-    int lo = 0, hi = a.nseq - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.cu_q[mid] <= row) lo = mid;
-        else hi = mid - 1;
-    }
-    const PromptSeq s = prompt_seq(a, lo, lane == 0);
-    if (row < s.q0 || row >= s.q0 + s.n) return;
-    const int seen = min(s.m, s.m - s.n + (int)(row - s.q0) + 1);
-    const uint16_t *qp = a.q.p + row * a.q.rs + (long)head * a.q.hs + lane * E;
-    const uint16_t *kp = a.k.p + (long)s.k0 * a.k.rs + (long)(head / a.group) * a.k.hs + lane * E;
-    const uint16_t *vp = a.v.p + (long)s.k0 * a.v.rs + (long)(head / a.group) * a.v.hs + lane * E;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
+__global__ void __launch_bounds__(pa::Cfg<D>::THREADS, 1)
+k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+            const __grid_constant__ CUtensorMap vmap, const PromptArgs a) {
+    using C = pa::Cfg<D>;
+    constexpr int NQ = C::NQ, NST = C::NST, PARTS = C::PARTS;
+    extern __shared__ __align__(1024) uint8_t pa_dyn[];
+    __shared__ __align__(8) uint64_t q_full, full[NST], empty[NST], checked[NST], s_full[2], p_full[2],
+        o_done[NQ];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag, poison, found_s[2], wsum[C::THREADS / 32];
+    // first key (from the first looked after, 1023: none) with a NaN, +inf, -inf in
+    // a dim, ten bits each; at most four tiles are looked after
+    __shared__ uint32_t first_bad[D];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- this CTA's rows: blocks of ROWS rows, a sequence's last block (the one
+    // with the most keys) first
+    const int head = (int)(blockIdx.x % (unsigned)a.heads), block = (int)(blockIdx.x / (unsigned)a.heads);
+    if (tid == 0) found_s[0] = -1;
+    {
+        int before = 0;
+        for (int s0 = 0; s0 < a.nseq && before <= block; s0 += C::THREADS) {
+            const int s = s0 + tid;
+            const int w = s < a.nseq ? (prompt_seq(a, s, blockIdx.x == 0).n + C::ROWS - 1) / C::ROWS : 0;
+            int incl = w;
 #pragma unroll
-    for (int i = 0; i < E; i++) { q[i] = bf16_f32(qp[i]) * a.zscale; o[i] = 0.f; }
-    for (int j = 0; j < seen; j++) {
-        float z = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; i++) z = fmaf(q[i], bf16_f32(kp[(long)j * a.k.rs + i]), z);
-#pragma unroll
-        for (int off = 16; off; off >>= 1) z += __shfl_xor_sync(0xffffffffu, z, off);
-        if (z > m) {
-            const float down = exp2f(m - z);
-            l *= down;
-#pragma unroll
-            for (int i = 0; i < E; i++) o[i] *= down;
-            m = z;
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += o;
+            }
+            if (lane == 31) wsum[warp] = incl;
+            __syncthreads();
+            int at = before + incl - w;
+            for (int k = 0; k < C::THREADS / 32; k++) {
+                if (k < warp) at += wsum[k];
+                before += wsum[k];
+            }
+            if (at <= block && block < at + w) { found_s[0] = s; found_s[1] = w - 1 - (block - at); }
+            __syncthreads();
         }
-        const float p = exp2f(z - m);
-        l += p;
-#pragma unroll
-        for (int i = 0; i < E; i++) o[i] = fmaf(p, bf16_f32(vp[(long)j * a.v.rs + i]), o[i]);
     }
-    uint16_t *op = a.out.p + row * a.out.rs + (long)head * a.out.hs + lane * E;
+    if (found_s[0] < 0) return;
+    const PromptSeq sq = prompt_seq(a, found_s[0], false);
+    const int r0 = found_s[1] * C::ROWS;                    // first row of the block, in the sequence
+    const int khead = head / a.group;
+    // key tiles of each query tile, and the first of them with keys that a row must not see
+    int nt[2] = {0, 0}, first_mask[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < E; i++) op[i] = bf16_bits(l == 0.f ? 0.f : o[i] / l);
+    for (int i = 0; i < NQ; i++) {
+        const int ra = r0 + i * pa::BM, rb = min(ra + pa::BM, sq.n);
+        if (ra < sq.n) {
+            nt[i] = (max(0, min(sq.m, sq.m - sq.n + rb)) + pa::BN - 1) / pa::BN;
+            first_mask[i] = max(0, min(sq.m, sq.m - sq.n + ra + 1)) / pa::BN;
+        }
+    }
+    const int ntmax = max(nt[0], nt[1]);
+    int mask_from = 0x7fffffff;                             // V tiles from here on are looked after
+#pragma unroll
+    for (int i = 0; i < NQ; i++)
+        if (nt[i] > 0) mask_from = min(mask_from, first_mask[i]);
+
+    for (int i = tid; i < D; i += C::THREADS) first_bad[i] = 0x3fffffffu;
+    if (tid == 0) {
+        mbar_init(&q_full, 1);
+        for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 3); mbar_init(&checked[s], 2); }   // products, two scanning warps
+        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
+        for (int i = 0; i < NQ; i++) mbar_init(&o_done[i], 1);
+        abort_flag = 0;
+        poison = 0;
+        fence_barrier_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    volatile int *ab = &abort_flag;
+    uint8_t *qs = pa_dyn + ((1024 - (smem_u32(pa_dyn) & 1023)) & 1023), *ring = qs + NQ * C::QTILE;
+
+    // The ring holds K 0, V 0, K 1, V 1, ... at NQ 2 and K 0, K 1, V 0, K 2, V 1,
+    // ... at NQ 1: the order in which they are used.  is_v, tile of ring entry e
+    // (each PARTS stages).
+    const int entries = 2 * ntmax;
+    auto entry = [&](int e, bool &is_v, int &tile) {
+        if (NQ == 2 || e == 0) { is_v = e & 1; tile = e >> 1; }
+        else if (e == entries - 1) { is_v = true; tile = ntmax - 1; }
+        else { is_v = !(e & 1); tile = is_v ? (e >> 1) - 1 : (e + 1) >> 1; }
+    };
+
+    if (warp == 0) {
+        if (lane == 0 && ntmax > 0) {   // ---- copies
+            mbar_arrive_expect_tx(&q_full, NQ * C::QTILE);
+            for (int i = 0; i < NQ; i++)
+                for (int p = 0; p < D / 64; p++)
+                    tma_load_3d(qs + i * C::QTILE + p * pa::PANEL, &qmap, p * 64, head, sq.q0 + r0 + i * pa::BM, &q_full);
+            int g = 0;
+            bool ok = true;
+            for (int e = 0; e < entries && ok; e++) {
+                bool is_v;
+                int tile;
+                entry(e, is_v, tile);
+                for (int part = 0; part < PARTS && ok; part++, g++) {
+                    const int s = g % NST;
+                    if (g >= NST && !(ok = mbar_wait(&empty[s], ((g / NST) - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT))) break;
+                    mbar_arrive_expect_tx(&full[s], C::STAGE);
+                    for (int p = 0; p < C::SPAN / 64; p++)
+                        tma_load_3d(ring + s * C::STAGE + p * pa::PANEL, is_v ? &vmap : &kmap, part * C::SPAN + p * 64, khead,
+                                    sq.k0 + tile * pa::BN, &full[s]);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && ntmax > 0) {   // ---- products
+            int g = 0;
+            bool ok = mbar_wait(&q_full, 0, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+            auto stage_wait = [&](int gg) {
+                ok = ok && mbar_wait(&full[gg % NST], (gg / NST) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+                tc_fence_after();
+            };
+            auto v_wait = [&](int gg, int tile) {
+                stage_wait(gg);
+                if (tile >= mask_from)
+                    ok = ok && mbar_wait(&checked[gg % NST], (gg / NST) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+            };
+            // S[buf] = Q[i] . K (stages gg ..)
+            auto mma_s = [&](int i, int buf, int gg, int part) {
+                const uint32_t kb = smem_u32(ring + (gg % NST) * C::STAGE);
+                const uint32_t qb = smem_u32(qs + i * C::QTILE) + part * (C::SPAN / 64) * pa::PANEL;
+#pragma unroll
+                for (int k = 0; k < C::SPAN / 16; k++) {
+                    const uint32_t off = (k >> 2) * pa::PANEL + (k & 3) * 32;
+                    tc_mma(tmem + buf * 128, umma_desc_sw128(qb + off), umma_desc_sw128(kb + off), C::IDESC_S, (part | k) != 0);
+                }
+            };
+            // O[i] (+)= P[buf] . V (stage gg)
+            auto mma_o = [&](int i, int buf, int gg, int part, bool acc) {
+                const uint32_t vb = smem_u32(ring + (gg % NST) * C::STAGE);
+#pragma unroll
+                for (int k = 0; k < pa::BN / 16; k++)
+                    tc_mma_ts(tmem + C::O_COL + i * D + part * C::SPAN, tmem + buf * 128 + k * 8,
+                              umma_desc_mn_sw128(vb + k * 2048, pa::PANEL), C::IDESC_O, acc || k != 0);
+            };
+            auto p_wait = [&](int buf, int use) {
+                ok = ok && mbar_wait(&p_full[buf], use & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+                tc_fence_after();
+            };
+            if constexpr (NQ == 2) {
+                stage_wait(0);
+                if (ok) {
+                    for (int i = 0; i < 2; i++)
+                        if (nt[i] > 0) { mma_s(i, i, 0, 0); tc_commit(&s_full[i]); }
+                    tc_commit(&empty[0]);
+                }
+                for (int j = 0; j < ntmax && ok; j++) {
+                    const int gv = 2 * j + 1, gk = 2 * j + 2;
+                    v_wait(gv, j);
+                    if (j + 1 < ntmax) stage_wait(gk);
+                    for (int i = 0; i < 2 && ok; i++) {
+                        if (j < nt[i]) {
+                            p_wait(i, j);
+                            if (!ok) break;
+                            mma_o(i, i, gv, 0, j > 0);
+                            tc_commit(&o_done[i]);
+                        }
+                        if (i == 1) tc_commit(&empty[gv % NST]);
+                        if (j + 1 < nt[i]) { mma_s(i, i, gk, 0); tc_commit(&s_full[i]); }
+                        if (i == 1 && j + 1 < ntmax) tc_commit(&empty[gk % NST]);
+                    }
+                }
+            } else {
+                auto do_s = [&](int j) {
+                    for (int part = 0; part < PARTS && ok; part++, g++) {
+                        stage_wait(g);
+                        if (!ok) return;
+                        mma_s(0, j & 1, g, part);
+                        tc_commit(&empty[g % NST]);
+                    }
+                    tc_commit(&s_full[j & 1]);
+                };
+                do_s(0);
+                for (int j = 0; j < ntmax && ok; j++) {
+                    if (j + 1 < ntmax) do_s(j + 1);
+                    if (!ok) break;
+                    p_wait(j & 1, j >> 1);
+                    for (int part = 0; part < PARTS && ok; part++, g++) {
+                        v_wait(g, j);
+                        if (!ok) break;
+                        mma_o(0, j & 1, g, part, j > 0);
+                        tc_commit(&empty[g % NST]);
+                    }
+                    if (ok) tc_commit(&o_done[0]);
+                }
+            }
+        }
+    } else if (warp < 4) {              // ---- V tiles with hidden keys
+        const int w64 = tid - 64;
+        int g = 0;
+        bool ok = true;
+        for (int e = 0; e < entries && ok; e++) {
+            bool is_v;
+            int tile;
+            entry(e, is_v, tile);
+            for (int part = 0; part < PARTS; part++, g++) {
+                const int s = g % NST;
+                const bool got = mbar_wait(&full[s], (g / NST) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+                ok = __all_sync(0xffffffffu, got);
+                if (!ok) break;
+                if (is_v && tile >= mask_from) {
+                    uint8_t *st = ring + s * C::STAGE;
+                    const int behind = sq.m - tile * pa::BN;        // rows from here on belong to no key
+                    // eight 16-byte pieces at a time: an exponent of all ones carries
+                    // into the sign bit
+                    for (int i = w64 * 16; i < C::STAGE; i += 8 * 64 * 16) {
+                        uint4 w[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) w[k] = lds128(st + i + k * 1024);
+                        if (behind < pa::BN) {
+#pragma unroll
+                            for (int k = 0; k < 8; k++)
+                                if ((((i + k * 1024) / 128) & 127) >= behind) {
+                                    w[k] = make_uint4(0, 0, 0, 0);
+                                    *(uint4 *)(st + i + k * 1024) = w[k];
+                                }
+                        }
+                        uint32_t bad = 0;
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            bad |= ((w[k].x & 0x7f807f80u) + 0x00800080u) | ((w[k].y & 0x7f807f80u) + 0x00800080u) |
+                                   ((w[k].z & 0x7f807f80u) + 0x00800080u) | ((w[k].w & 0x7f807f80u) + 0x00800080u);
+                        if (!(bad & 0x80008000u)) continue;
+#pragma unroll 1
+                        for (int k = 0; k < 8; k++) {
+                            const int at = i + k * 1024, r = (at / 128) & 127;
+                            // the piece's place in its row is swizzled by the row
+                            const int d0 = part * C::SPAN + (at / pa::PANEL) * 64 + (((at >> 4) & 7) ^ (r & 7)) * 8;
+                            uint16_t *h = (uint16_t *)(st + at);
+                            for (int u = 0; u < 8; u++) {
+                                const uint16_t x = h[u];
+                                if ((x & 0x7f80) != 0x7f80) continue;
+                                h[u] = 0;
+                                const int sh = ((x & 0x7f) ? 0 : (x >> 15) ? 2 : 1) * 10;
+                                const uint32_t key = (uint32_t)((tile - mask_from) * pa::BN + r);
+                                uint32_t old = first_bad[d0 + u], was;
+                                while (key < ((old >> sh) & 1023u)) {
+                                    was = old;
+                                    old = atomicCAS(&first_bad[d0 + u], was, (was & ~(1023u << sh)) | (key << sh));
+                                    if (old == was) break;
+                                }
+                                poison = 1;
+                            }
+                        }
+                    }
+                    static_assert(C::STAGE % (8 * 64 * 16) == 0, "whole batches of pieces");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&checked[s]);
+                    mbar_arrive(&empty[s]);
+                }
+            }
+        }
+    } else {                            // ---- softmax, one row a thread
+        const int i = (warp - 4) >> 2;                      // query tile
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int rt = (warp & 3) * 32 + lane, row = r0 + i * pa::BM + rt;      // row in the sequence
+        const int nti = nt[i];
+        const int seen = max(0, min(sq.m, sq.m - sq.n + min(row, sq.n - 1) + 1));   // keys that it sees
+        const uint32_t o_col = tmem + lanes + C::O_COL + i * D;
+        float m = -INFINITY, l = 0.f;
+        const float raise = pa::RAISE / a.zscale;
+        bool ok = true;
+        for (int j = 0; j < nti; j++) {
+            const int buf = NQ == 2 ? i : (j & 1), use = NQ == 2 ? j : (j >> 1);
+            const bool got = mbar_wait(&s_full[buf], use & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+            ok = __all_sync(0xffffffffu, got);
+            if (!ok) break;
+            tc_fence_after();
+            float v[128];
+            tc_ld128(tmem + lanes + buf * 128, v);
+            if (j >= first_mask[i]) {
+                const int lim = seen - j * pa::BN;
+#pragma unroll
+                for (int c = 0; c < 128; c++) v[c] = c < lim ? v[c] : -INFINITY;
+            }
+            float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int c = 4; c < 128; c += 4)
+#pragma unroll
+                for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], v[c + u]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool up = top > m + raise;
+            if (__any_sync(0xffffffffu, up)) {
+                const float down = !up ? 1.0f : m == -INFINITY ? 0.f : pa_ex2((m - top) * a.zscale);
+                if (up) m = top;
+                l *= down;
+                if (j > 0) {
+                    const bool done = mbar_wait(&o_done[NQ == 2 ? i : 0], (j - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+                    ok = __all_sync(0xffffffffu, done);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tc_ld32(o_col + c, o);
+#pragma unroll
+                        for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * down);
+                        tc_st32(o_col + c, o);
+                    }
+                }
+            }
+            const float mz = m == -INFINITY ? 0.f : m * a.zscale;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int u = 0; u < 32; u += 2) {
+                    const float p0 = pa_ex2(fmaf(v[c + u], a.zscale, -mz)), p1 = pa_ex2(fmaf(v[c + u + 1], a.zscale, -mz));
+                    sum[u & 2] += p0;
+                    sum[(u & 2) + 1] += p1;
+                    pk[u / 2] = pa_pack(p0, p1);
+                }
+                tc_st16(tmem + lanes + buf * 128 + c / 2, pk);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if (NQ == 1 && j > 0) {
+                // every phase of o_done is waited for (at NQ 2 the S tile of j is
+                // behind the product of j - 1 on the same pipe, so it has passed)
+                const bool done = mbar_wait(&o_done[0], (j - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+                ok = __all_sync(0xffffffffu, done);
+                if (!ok) break;
+            }
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[buf]);
+        }
+        if (ok && nti > 0) {
+            const bool done = mbar_wait(&o_done[NQ == 2 ? i : 0], (nti - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+            ok = __all_sync(0xffffffffu, done);
+            tc_fence_after();
+        }
+        if (ok) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            uint16_t *op = a.out.p + (long)(sq.q0 + row) * a.out.rs + (long)head * a.out.hs;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (nti > 0) tc_ld32(o_col + c, o);
+                if (*(volatile int *)&poison) {
+#pragma unroll
+                    for (int u = 0; u < 32; u++) {
+                        float x = __uint_as_float(o[u]);
+                        const uint32_t f = first_bad[c + u];
+                        const int rel = seen - mask_from * pa::BN;       // looked-after keys that the row sees
+                        if (rel > (int)(f & 1023u)) x = __int_as_float(0x7fc00000);
+                        if (rel > (int)((f >> 10) & 1023u)) x += INFINITY;
+                        if (rel > (int)(f >> 20)) x -= INFINITY;
+                        o[u] = __float_as_uint(x);
+                    }
+                }
+                if (row < sq.n) {
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            w[u] = nti > 0 ? pa_pack(__uint_as_float(o[8 * h + 2 * u]) * inv,
+                                                     __uint_as_float(o[8 * h + 2 * u + 1]) * inv) : 0u;
+                        *(uint4 *)(op + c + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 }  // namespace apus
 using namespace apus;
+
+// 3-D BF16 tensor map of rows of heads (dims, heads, rows): boxes of 64 dims of
+// one head of 128 rows in the 128-byte swizzle; zeros past the last row.
+static int pa_map(CUtensorMap *m, const ApusHeadRows *r, size_t dim) {
+    static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+    if (!enc) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            gcuda_set_error("prompt_attn: no tensor map encoder");
+            return -1;
+        }
+        enc = (PFN_cuTensorMapEncodeTiled_v12000)p;
+    }
+    // the stride of an axis of one is not looked at, but has to be a valid one
+    const cuuint64_t dims[3] = {dim, r->heads, r->rows};
+    const cuuint64_t strides[2] = {r->heads > 1 ? r->head_stride * 2 : dim * 2, r->rows > 1 ? r->row_stride * 2 : dim * 2};
+    const cuuint32_t box[3] = {64, 1, 128}, es[3] = {1, 1, 1};
+    if (enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, r->p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        gcuda_set_error("prompt_attn: tensor map of %zu rows of %zu heads, strides %zu, %zu", r->rows, r->heads,
+                        r->row_stride, r->head_stride);
+        return -1;
+    }
+    return 0;
+}
+
+template <int D>
+static int pa_launch(const PromptArgs &a, const ApusHeadRows *q, const ApusHeadRows *k, const ApusHeadRows *v,
+                     cudaStream_t st) {
+    using C = pa::Cfg<D>;
+    const long blocks = ((long)a.rows_q / C::ROWS + a.nseq) * a.heads;
+    if (blocks >= (1l << 31)) { gcuda_set_error("prompt_attn: %d rows of %d heads", a.rows_q, a.heads); return -1; }
+    CUtensorMap qm, km, vm;
+    if (pa_map(&qm, q, D) || pa_map(&km, k, D) || pa_map(&vm, v, D)) return -1;
+    if (gcuda_smem_limit_once((const void *)k_prompt_tc<D>, C::SMEM)) return -1;
+    k_prompt_tc<D><<<(unsigned)blocks, C::THREADS, C::SMEM, st>>>(qm, km, vm, a);
+    return gcuda_check(cudaGetLastError(), "prompt_attn launch");
+}
 
 extern "C" int apus_gcuda_prompt_attn_dev(const ApusPromptBatch *batch, const ApusHeadRows *q, const ApusHeadRows *k,
                                           const ApusHeadRows *v, const ApusHeadRows *out, size_t dim, float scale,
                                           void *stream) {
     const char *what = "prompt_attn";
     if (!batch) { gcuda_set_error("%s: no batch given", what); return -1; }
-    if (attn_check_dim(what, dim)) return -1;
+    if (attn_check_dim(what, dim) || attn_check_scale(what, scale)) return -1;
     if (attn_check_rows(what, q, dim, false) || attn_check_rows(what, k, dim, false) ||
         attn_check_rows(what, v, dim, false) || attn_check_rows(what, out, dim, true))
         return -1;
@@ -100,12 +545,12 @@ extern "C" int apus_gcuda_prompt_attn_dev(const ApusPromptBatch *batch, const Ap
     PromptArgs a{batch->cu_q, batch->cu_k, (int)batch->nseq, (int)q->rows, (int)k->rows, (int)batch->max_rows,
                  rows_view(q), rows_view(k), rows_view(v), rows_view(out), (int)q->heads, (int)(q->heads / k->heads),
                  scale * 1.4426950408889634f};
-    const dim3 grid((unsigned)((q->rows + 3) / 4), (unsigned)q->heads);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (dim == 64) k_prompt_rows<64><<<grid, 128, 0, st>>>(a);
-    else if (dim == 128) k_prompt_rows<128><<<grid, 128, 0, st>>>(a);
-    else k_prompt_rows<256><<<grid, 128, 0, st>>>(a);
-    return gcuda_check(cudaGetLastError(), "prompt_attn launch");
+    // without keys every row gives zeros; the tensor maps need a row to stand on
+    ApusHeadRows kk = *k, vv = *v;
+    if (!k->rows) { kk = vv = *q; kk.heads = vv.heads = 1; }
+    if (dim == 64) return pa_launch<64>(a, q, &kk, &vv, (cudaStream_t)stream);
+    if (dim == 128) return pa_launch<128>(a, q, &kk, &vv, (cudaStream_t)stream);
+    return pa_launch<256>(a, q, &kk, &vv, (cudaStream_t)stream);
 }
 
 int prompt_attn_error_read_and_clear(void) {

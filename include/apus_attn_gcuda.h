@@ -11,6 +11,7 @@
  *   - No allocation, no synchronisation, no state kept between calls: every
  *     entry can be captured into a CUDA graph, and calls on different streams
  *     may overlap as long as their outputs and workspaces do not.
+ *   - Scales are positive and finite; head dims are 64, 128 or 256.
  *   - The structs are read during the call; the device arrays they point to
  *     are read by the kernels, so they must live until those have run.
  *   - What the host cannot see is checked on the device: a page id, a length

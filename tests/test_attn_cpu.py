@@ -46,6 +46,7 @@ BAD_ROWS = [dict(p=0), dict(p=AT + 8), dict(row_stride=260), dict(head_stride=13
             dict(row_stride=1 << 31)]
 BAD_CACHE = [dict(dim=96), dict(dim=0), dict(dim=512), dict(heads=0), dict(pages=0), dict(pages=AT + 4),
              dict(num_pages=1 << 31)]
+BAD_SCALES = [0.0, -0.5, float("nan"), float("inf")]
 BAD_BATCH = [dict(cu_rows=0), dict(kv_len=0), dict(page_table=0), dict(max_len=257), dict(nseq=70000),
              dict(max_rows=1 << 31), dict(table_stride=1 << 31)]
 
@@ -72,9 +73,9 @@ def test_read_refuses_overlapping_outputs():
     refused(G.apus_gcuda_kv4_read_dev(cache(), batch(), rows(), over, None), "overlap")
 
 
-def attn(c=None, b=None, q=None, out=None, sel=None, stride=0, pool=0, work=AT, nbytes=1 << 30):
+def attn(c=None, b=None, q=None, out=None, sel=None, stride=0, pool=0, work=AT, nbytes=1 << 30, scale=0.1):
     return G.apus_gcuda_kv4_attn_dev(c or cache(), b or batch(), q or rows(heads=4, row_stride=512),
-                                     out or rows(heads=4, row_stride=512), 0.1, sel, stride, pool, work, nbytes, None)
+                                     out or rows(heads=4, row_stride=512), scale, sel, stride, pool, work, nbytes, None)
 
 
 def test_attention_refused():
@@ -91,6 +92,8 @@ def test_attention_refused():
     refused(attn(out=rows(heads=2)), "out")
     refused(attn(out=rows(heads=4, row_stride=512, rows=3)), "out")
     refused(attn(out=rows(heads=4, row_stride=128)), "overlap")
+    for scale in BAD_SCALES:
+        refused(attn(scale=scale), "scale")
     refused(attn(sel=AT, stride=8, pool=0), "pools")
     refused(attn(sel=AT, stride=8, pool=129), "pools")
     refused(attn(sel=AT, stride=1 << 31, pool=4), "pools")
@@ -105,11 +108,13 @@ def test_attention_refused():
 
 
 def test_prompt_refused():
-    def call(b=None, q=None, k=None, v=None, out=None, dim=128):
+    def call(b=None, q=None, k=None, v=None, out=None, dim=128, scale=0.1):
         wide = rows(heads=4, row_stride=512)
-        return G.apus_gcuda_prompt_attn_dev(b or prompt(), q or wide, k or rows(), v or rows(), out or wide, dim, 0.1, None)
+        return G.apus_gcuda_prompt_attn_dev(b or prompt(), q or wide, k or rows(), v or rows(), out or wide, dim, scale, None)
     for dim in (0, 32, 96, 512):
         refused(call(dim=dim), "prompt_attn", str(dim))
+    for scale in BAD_SCALES:
+        refused(call(scale=scale), "scale")
     for bad in (dict(cu_q=0), dict(cu_k=0), dict(nseq=70000), dict(max_rows=1 << 31)):
         refused(call(b=prompt(**bad)), "prompt_attn")
     for bad in BAD_ROWS:
