@@ -14,10 +14,13 @@
 // Bound: at dim 256 the products (2048 tensor cycles a tile of 128 x 128), at
 // dim 128 products and exponentials alike (1024 tensor cycles; 16384
 // exponentials at 16 a cycle), at dim 64 the exponentials.
-// So two query tiles share an SM up to dim 128: one tile's softmax runs under
-// the other's products.  At dim 256 the accumulator of one tile fills half of
-// TMEM and two S tiles the other half: the next tile's S is computed under this
-// tile's softmax.
+// Up to dim 128 two query tiles share an SM, so that each K and V tile serves 256
+// rows and one tile's softmax runs under the other's products.  S has one place
+// in TMEM, which the softmax frees as soon as it holds the scores in registers; P
+// has a place of its own.  So the next S is there when a softmax ends.  (With P
+// written over S, a query tile waited 1400 of 3700 cycles for its own products;
+// two S tiles of 64 keys made the products of S, which read 128 rows of Q for 64
+// keys, the bound.)
 //
 // Roles: warp 0 copies, warp 1 issues the products, warps 2-3 look after V tiles
 // with keys that some row must not see, warps 4.. are one softmax group of 128
@@ -58,7 +61,7 @@ APUS_DEV PromptSeq prompt_seq(const PromptArgs &a, int s, bool report) {
 }
 
 namespace pa {
-constexpr int BM = 128, BN = 128;               // query rows of a tile, keys of a tile
+constexpr int BM = 128, BN = 128;               // query rows of a tile, keys of a K or V tile
 constexpr int PANEL = 128 * 128;                // bytes of 128 rows of 64 dims
 template <int D> struct Cfg {
     static constexpr int NQ = D == 256 ? 1 : 2;             // query tiles of a CTA
@@ -70,7 +73,7 @@ template <int D> struct Cfg {
     static constexpr int NST = D == 256 ? 5 : D == 128 ? 4 : 8;
     static constexpr int SMEM = NQ * QTILE + NST * STAGE + 1024;
     static constexpr int ROWS = NQ * BM;
-    static constexpr int O_COL = 256;                       // TMEM: S tiles at 0 and 128, O from 256
+    static constexpr int P_COL = 128, O_COL = 256;          // TMEM: S from 0, each query tile's P and O
     // D f32, A and B BF16, N >> 3 at bit 17, M >> 4 at bit 24; V has its dims
     // (N) contiguous: bit 16
     static constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
@@ -99,14 +102,16 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     using C = pa::Cfg<D>;
     constexpr int NQ = C::NQ, NST = C::NST, PARTS = C::PARTS;
     extern __shared__ __align__(1024) uint8_t pa_dyn[];
-    __shared__ __align__(8) uint64_t q_full, full[NST], empty[NST], checked[NST], s_full[2], p_full[2],
+    __shared__ __align__(8) uint64_t q_full, full[NST], empty[NST], checked[NST], s_free, s_full[NQ], p_full[NQ],
         o_done[NQ];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, poison, found_s[2], wsum[C::THREADS / 32];
     // first key (from the first looked after, 1023: none) with a NaN, +inf, -inf in
     // a dim, ten bits each; at most four tiles are looked after
     __shared__ uint32_t first_bad[D];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (a shuffle tells the compiler that it is the same for the warp, so that the
+    // products' operands stay in uniform registers)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     // ---- this CTA's rows: blocks of ROWS rows, a sequence's last block (the one
     // with the most keys) first
@@ -138,28 +143,26 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     const PromptSeq sq = prompt_seq(a, found_s[0], false);
     const int r0 = found_s[1] * C::ROWS;                    // first row of the block, in the sequence
     const int khead = head / a.group;
-    // key tiles of each query tile, and the first of them with keys that a row must not see
-    int nt[2] = {0, 0}, first_mask[2] = {0, 0};
+    // key tiles of each query tile, the first of them with keys that a row must
+    // not see, and the first that is looked after
+    int nt[2] = {0, 0}, first_mask[2] = {0, 0}, mask_from = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
         const int ra = r0 + i * pa::BM, rb = min(ra + pa::BM, sq.n);
         if (ra < sq.n) {
             nt[i] = (max(0, min(sq.m, sq.m - sq.n + rb)) + pa::BN - 1) / pa::BN;
             first_mask[i] = max(0, min(sq.m, sq.m - sq.n + ra + 1)) / pa::BN;
+            if (nt[i] > 0) mask_from = min(mask_from, first_mask[i]);
         }
     }
     const int ntmax = max(nt[0], nt[1]);
-    int mask_from = 0x7fffffff;                             // V tiles from here on are looked after
-#pragma unroll
-    for (int i = 0; i < NQ; i++)
-        if (nt[i] > 0) mask_from = min(mask_from, first_mask[i]);
 
     for (int i = tid; i < D; i += C::THREADS) first_bad[i] = 0x3fffffffu;
     if (tid == 0) {
         mbar_init(&q_full, 1);
         for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 3); mbar_init(&checked[s], 2); }   // products, two scanning warps
-        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); }
-        for (int i = 0; i < NQ; i++) mbar_init(&o_done[i], 1);
+        mbar_init(&s_free, 128);
+        for (int i = 0; i < NQ; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_done[i], 1); }
         abort_flag = 0;
         poison = 0;
         fence_barrier_init();
@@ -172,19 +175,21 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     volatile int *ab = &abort_flag;
     uint8_t *qs = pa_dyn + ((1024 - (smem_u32(pa_dyn) & 1023)) & 1023), *ring = qs + NQ * C::QTILE;
 
-    // The ring holds K 0, V 0, K 1, V 1, ... at NQ 2 and K 0, K 1, V 0, K 2, V 1,
-    // ... at NQ 1: the order in which they are used.  is_v, tile of ring entry e
-    // (each PARTS stages).
+    // The ring holds K 0, K 1, V 0, K 2, V 1, ..., the order in which they are
+    // used.  is_v, tile of ring entry e (each PARTS stages).
     const int entries = 2 * ntmax;
     auto entry = [&](int e, bool &is_v, int &tile) {
-        if (NQ == 2 || e == 0) { is_v = e & 1; tile = e >> 1; }
+        if (e == 0) { is_v = false; tile = 0; }
         else if (e == entries - 1) { is_v = true; tile = ntmax - 1; }
         else { is_v = !(e & 1); tile = is_v ? (e >> 1) - 1 : (e + 1) >> 1; }
     };
+    // ... and the first stage of a K or V tile
+    auto k_stage = [&](int tile) { return (tile == 0 ? 0 : 2 * tile - 1) * PARTS; };
+    auto v_stage = [&](int tile) { return (tile == ntmax - 1 ? entries - 1 : 2 * tile + 2) * PARTS; };
 
     if (warp == 0) {
         if (lane == 0 && ntmax > 0) {   // ---- copies
@@ -209,87 +214,75 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && ntmax > 0) {   // ---- products
-            int g = 0;
-            bool ok = mbar_wait(&q_full, 0, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-            auto stage_wait = [&](int gg) {
-                ok = ok && mbar_wait(&full[gg % NST], (gg / NST) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+        if (ntmax > 0) {                // ---- products (the whole warp, one elected lane issuing)
+            const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
+            const int mf = __shfl_sync(0xffffffffu, mask_from, 0), total = n0 + n1;
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int parity) {
+                if (!__all_sync(0xffffffffu, ok && mbar_try_wait(bar, parity)))
+                    ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
                 tc_fence_after();
             };
-            auto v_wait = [&](int gg, int tile) {
-                stage_wait(gg);
-                if (tile >= mask_from)
-                    ok = ok && mbar_wait(&checked[gg % NST], (gg / NST) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-            };
-            // S[buf] = Q[i] . K (stages gg ..)
-            auto mma_s = [&](int i, int buf, int gg, int part) {
-                const uint32_t kb = smem_u32(ring + (gg % NST) * C::STAGE);
-                const uint32_t qb = smem_u32(qs + i * C::QTILE) + part * (C::SPAN / 64) * pa::PANEL;
+            // S = Q[i] . K tile j; the last query tile to use the K tile frees it
+            auto mma_s = [&](int i, int j, bool frees) {
 #pragma unroll
-                for (int k = 0; k < C::SPAN / 16; k++) {
-                    const uint32_t off = (k >> 2) * pa::PANEL + (k & 3) * 32;
-                    tc_mma(tmem + buf * 128, umma_desc_sw128(qb + off), umma_desc_sw128(kb + off), C::IDESC_S, (part | k) != 0);
-                }
-            };
-            // O[i] (+)= P[buf] . V (stage gg)
-            auto mma_o = [&](int i, int buf, int gg, int part, bool acc) {
-                const uint32_t vb = smem_u32(ring + (gg % NST) * C::STAGE);
+                for (int part = 0; part < PARTS; part++) {
+                    const int gg = k_stage(j) + part;
+                    wait(&full[gg % NST], (gg / NST) & 1);
+                    if (!ok) return;
+                    const uint32_t kb = smem_u32(ring + (gg % NST) * C::STAGE);
+                    const uint32_t qb = smem_u32(qs + i * C::QTILE) + part * (C::SPAN / 64) * pa::PANEL;
 #pragma unroll
-                for (int k = 0; k < pa::BN / 16; k++)
-                    tc_mma_ts(tmem + C::O_COL + i * D + part * C::SPAN, tmem + buf * 128 + k * 8,
-                              umma_desc_mn_sw128(vb + k * 2048, pa::PANEL), C::IDESC_O, acc || k != 0);
-            };
-            auto p_wait = [&](int buf, int use) {
-                ok = ok && mbar_wait(&p_full[buf], use & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-                tc_fence_after();
-            };
-            if constexpr (NQ == 2) {
-                stage_wait(0);
-                if (ok) {
-                    for (int i = 0; i < 2; i++)
-                        if (nt[i] > 0) { mma_s(i, i, 0, 0); tc_commit(&s_full[i]); }
-                    tc_commit(&empty[0]);
-                }
-                for (int j = 0; j < ntmax && ok; j++) {
-                    const int gv = 2 * j + 1, gk = 2 * j + 2;
-                    v_wait(gv, j);
-                    if (j + 1 < ntmax) stage_wait(gk);
-                    for (int i = 0; i < 2 && ok; i++) {
-                        if (j < nt[i]) {
-                            p_wait(i, j);
-                            if (!ok) break;
-                            mma_o(i, i, gv, 0, j > 0);
-                            tc_commit(&o_done[i]);
-                        }
-                        if (i == 1) tc_commit(&empty[gv % NST]);
-                        if (j + 1 < nt[i]) { mma_s(i, i, gk, 0); tc_commit(&s_full[i]); }
-                        if (i == 1 && j + 1 < ntmax) tc_commit(&empty[gk % NST]);
+                    for (int k = 0; k < C::SPAN / 16; k++) {
+                        const uint32_t off = (k >> 2) * pa::PANEL + (k & 3) * 32;
+                        tc_mma_warp(tmem, umma_desc_sw128(qb + off), umma_desc_sw128(kb + off), C::IDESC_S, (part | k) != 0);
                     }
+                    if (frees) tc_commit_warp(&empty[gg % NST]);
                 }
-            } else {
-                auto do_s = [&](int j) {
-                    for (int part = 0; part < PARTS && ok; part++, g++) {
-                        stage_wait(g);
-                        if (!ok) return;
-                        mma_s(0, j & 1, g, part);
-                        tc_commit(&empty[g % NST]);
-                    }
-                    tc_commit(&s_full[j & 1]);
-                };
-                do_s(0);
-                for (int j = 0; j < ntmax && ok; j++) {
-                    if (j + 1 < ntmax) do_s(j + 1);
+                tc_commit_warp(&s_full[i]);
+            };
+            // O[i] (+)= P[i] . V tile j
+            auto mma_o = [&](int i, int j, bool frees) {
+#pragma unroll
+                for (int part = 0; part < PARTS; part++) {
+                    const int gg = v_stage(j) + part;
+                    wait(&full[gg % NST], (gg / NST) & 1);
+                    if (j >= mf) wait(&checked[gg % NST], (gg / NST) & 1);
+                    if (!ok) return;
+                    const uint32_t vb = smem_u32(ring + (gg % NST) * C::STAGE);
+#pragma unroll
+                    for (int k = 0; k < pa::BN / 16; k++)
+                        tc_mma_ts_warp(tmem + C::O_COL + i * D + part * C::SPAN, tmem + C::P_COL + i * 64 + k * 8,
+                                       umma_desc_mn_sw128(vb + k * 2048, pa::PANEL), C::IDESC_O, j > 0 || k != 0);
+                    if (frees) tc_commit_warp(&empty[gg % NST]);
+                }
+                tc_commit_warp(&o_done[i]);
+            };
+            // The uses of S: tile j of query tile 0, of query tile 1 (while they have
+            // tiles left), then j + 1.  S is free again as soon as the softmax has it
+            // in registers, so the products of S run NQ + 1 uses ahead of those of O:
+            // the softmax that ends finds its next S there.
+            int si = n0 > 0 ? 0 : 1, sj = 0, su = 0;
+            auto next_s = [&]() {
+                if (su >= total) return;
+                if (su > 0) wait(&s_free, (su - 1) & 1);
+                if (!ok) return;
+                const bool more = si == 0 && sj < n1;       // query tile 1 follows with the same K tile
+                mma_s(si, sj, !more);
+                if (more) si = 1;
+                else { sj++; si = sj < n0 ? 0 : 1; }
+                su++;
+            };
+            wait(&q_full, 0);
+            for (int k = 0; k <= NQ && ok; k++) next_s();
+            for (int j = 0; j < ntmax && ok; j++)
+                for (int i = 0; i < NQ && ok; i++) {
+                    if (j >= (i == 0 ? n0 : n1)) continue;
+                    wait(&p_full[i], j & 1);
                     if (!ok) break;
-                    p_wait(j & 1, j >> 1);
-                    for (int part = 0; part < PARTS && ok; part++, g++) {
-                        v_wait(g, j);
-                        if (!ok) break;
-                        mma_o(0, j & 1, g, part, j > 0);
-                        tc_commit(&empty[g % NST]);
-                    }
-                    if (ok) tc_commit(&o_done[0]);
+                    mma_o(i, j, i == 1 || j >= n1);
+                    if (ok) next_s();
                 }
-            }
         }
     } else if (warp < 4) {              // ---- V tiles with hidden keys
         const int w64 = tid - 64;
@@ -365,18 +358,22 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
         const int rt = (warp & 3) * 32 + lane, row = r0 + i * pa::BM + rt;      // row in the sequence
         const int nti = nt[i];
         const int seen = max(0, min(sq.m, sq.m - sq.n + min(row, sq.n - 1) + 1));   // keys that it sees
-        const uint32_t o_col = tmem + lanes + C::O_COL + i * D;
+        const uint32_t p_col = tmem + lanes + C::P_COL + i * 64, o_col = tmem + lanes + C::O_COL + i * D;
         float m = -INFINITY, l = 0.f;
         const float raise = pa::RAISE / a.zscale;
         bool ok = true;
-        for (int j = 0; j < nti; j++) {
-            const int buf = NQ == 2 ? i : (j & 1), use = NQ == 2 ? j : (j >> 1);
-            const bool got = mbar_wait(&s_full[buf], use & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-            ok = __all_sync(0xffffffffu, got);
-            if (!ok) break;
+        auto wait = [&](uint64_t *bar, int parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
             tc_fence_after();
+        };
+        for (int j = 0; j < nti; j++) {
+            wait(&s_full[i], j & 1);
+            if (!ok) break;
             float v[128];
-            tc_ld128(tmem + lanes + buf * 128, v);
+            tc_ld128(tmem + lanes, v);
+            tc_fence_before();
+            mbar_arrive(&s_free);
             if (j >= first_mask[i]) {
                 const int lim = seen - j * pa::BN;
 #pragma unroll
@@ -389,15 +386,16 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], v[c + u]);
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool up = top > m + raise;
+            // P's place is read by the product of j - 1 until that is done
+            if (j > 0) {
+                wait(&o_done[i], (j - 1) & 1);
+                if (!ok) break;
+            }
             if (__any_sync(0xffffffffu, up)) {
                 const float down = !up ? 1.0f : m == -INFINITY ? 0.f : pa_ex2((m - top) * a.zscale);
                 if (up) m = top;
                 l *= down;
                 if (j > 0) {
-                    const bool done = mbar_wait(&o_done[NQ == 2 ? i : 0], (j - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-                    ok = __all_sync(0xffffffffu, done);
-                    if (!ok) break;
-                    tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
@@ -420,25 +418,14 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                     sum[(u & 2) + 1] += p1;
                     pk[u / 2] = pa_pack(p0, p1);
                 }
-                tc_st16(tmem + lanes + buf * 128 + c / 2, pk);
+                tc_st16(p_col + c / 2, pk);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if (NQ == 1 && j > 0) {
-                // every phase of o_done is waited for (at NQ 2 the S tile of j is
-                // behind the product of j - 1 on the same pipe, so it has passed)
-                const bool done = mbar_wait(&o_done[0], (j - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-                ok = __all_sync(0xffffffffu, done);
-                if (!ok) break;
-            }
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_full[buf]);
+            mbar_arrive(&p_full[i]);
         }
-        if (ok && nti > 0) {
-            const bool done = mbar_wait(&o_done[NQ == 2 ? i : 0], (nti - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-            ok = __all_sync(0xffffffffu, done);
-            tc_fence_after();
-        }
+        if (ok && nti > 0) wait(&o_done[i], (nti - 1) & 1);
         if (ok) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             uint16_t *op = a.out.p + (long)(sq.q0 + row) * a.out.rs + (long)head * a.out.hs;
