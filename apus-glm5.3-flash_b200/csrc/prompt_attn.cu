@@ -22,9 +22,10 @@
 // two S tiles of 64 keys made the products of S, which read 128 rows of Q for 64
 // keys, the bound.)
 //
-// Roles: warp 0 copies, warp 1 issues the products, warps 2-3 look after V tiles
-// with keys that some row must not see, warps 4.. are one softmax group of 128
-// threads (a row each) a query tile.  The maximum is raised, and O rescaled, only
+// Roles: warp 0 copies, warp 1 issues the products of S, warp 3 those of O (one
+// warp for both spent 3400 cycles on issuing 2048 cycles of products), warp 2
+// looks after V tiles with keys that some row must not see, warps 4.. are one
+// softmax group of 128 threads (a row each) a query tile.  The maximum is raised, and O rescaled, only
 // when a score passes it by more than 2^8, so almost never.
 //
 // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value would
@@ -73,7 +74,7 @@ template <int D> struct Cfg {
     static constexpr int NST = D == 256 ? 5 : D == 128 ? 4 : 8;
     static constexpr int SMEM = NQ * QTILE + NST * STAGE + 1024;
     static constexpr int ROWS = NQ * BM;
-    static constexpr int P_COL = 128, O_COL = 256;          // TMEM: S from 0, each query tile's P and O
+    static constexpr int P_COL = 128, O_COL = 256;          // TMEM: S from 0, two P, each query tile's O
     // D f32, A and B BF16, N >> 3 at bit 17, M >> 4 at bit 24; V has its dims
     // (N) contiguous: bit 16
     static constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
@@ -102,8 +103,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     using C = pa::Cfg<D>;
     constexpr int NQ = C::NQ, NST = C::NST, PARTS = C::PARTS;
     extern __shared__ __align__(1024) uint8_t pa_dyn[];
-    __shared__ __align__(8) uint64_t q_full, full[NST], empty[NST], checked[NST], s_free, s_full[NQ], p_full[NQ],
-        o_done[NQ];
+    __shared__ __align__(8) uint64_t q_full, full[NST], empty[NST], checked[NST], s_free, s_full[2], p_full[2], o_done[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, poison, found_s[2], wsum[C::THREADS / 32];
     // first key (from the first looked after, 1023: none) with a NaN, +inf, -inf in
@@ -160,9 +160,9 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     for (int i = tid; i < D; i += C::THREADS) first_bad[i] = 0x3fffffffu;
     if (tid == 0) {
         mbar_init(&q_full, 1);
-        for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 3); mbar_init(&checked[s], 2); }   // products, two scanning warps
+        for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&checked[s], 1); }   // empty: products, scan
         mbar_init(&s_free, 128);
-        for (int i = 0; i < NQ; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_done[i], 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_done[i], 1); }
         abort_flag = 0;
         poison = 0;
         fence_barrier_init();
@@ -182,15 +182,15 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     // The ring holds K 0, K 1, V 0, K 2, V 1, ..., the order in which they are
     // used.  is_v, tile of ring entry e (each PARTS stages).
     const int entries = 2 * ntmax;
+    // The P of query tile i and key tile j: one place a query tile, or (NQ 1) two
+    // that take turns; its barriers p_full and o_done and how often they were used.
+    auto p_at = [](int i, int j) { return NQ == 2 ? i : (j & 1); };
+    auto p_use = [](int j) { return NQ == 2 ? j : (j >> 1); };
     auto entry = [&](int e, bool &is_v, int &tile) {
         if (e == 0) { is_v = false; tile = 0; }
         else if (e == entries - 1) { is_v = true; tile = ntmax - 1; }
         else { is_v = !(e & 1); tile = is_v ? (e >> 1) - 1 : (e + 1) >> 1; }
     };
-    // ... and the first stage of a K or V tile
-    auto k_stage = [&](int tile) { return (tile == 0 ? 0 : 2 * tile - 1) * PARTS; };
-    auto v_stage = [&](int tile) { return (tile == ntmax - 1 ? entries - 1 : 2 * tile + 2) * PARTS; };
-
     if (warp == 0) {
         if (lane == 0 && ntmax > 0) {   // ---- copies
             mbar_arrive_expect_tx(&q_full, NQ * C::QTILE);
@@ -213,79 +213,73 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 }
             }
         }
-    } else if (warp == 1) {
-        if (ntmax > 0) {                // ---- products (the whole warp, one elected lane issuing)
-            const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
-            const int mf = __shfl_sync(0xffffffffu, mask_from, 0), total = n0 + n1;
-            bool ok = true;
-            auto wait = [&](uint64_t *bar, int parity) {
-                if (!__all_sync(0xffffffffu, ok && mbar_try_wait(bar, parity)))
-                    ok = __all_sync(0xffffffffu, ok && mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
+    } else if (warp == 1) {             // ---- S = Q . K^T (the whole warp, one elected lane issuing)
+        const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, int parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
+        };
+        if (ntmax > 0) wait(&q_full, 0);
+        // The uses of S: key tile j of query tile 0, then of query tile 1, while they
+        // have tiles left.  S is free again as soon as a softmax has it in registers,
+        // so the softmax that ends finds its next S there.
+        int use = 0;
+        for (int j = 0; j < max(n0, n1) && ok; j++)
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                if (!ok || j >= (i == 0 ? n0 : n1)) continue;
+                const bool first = i == 0 || j >= n0, last = i == NQ - 1 || j >= n1;   // to use this K tile
+                if (use > 0) wait(&s_free, (use - 1) & 1);
                 tc_fence_after();
-            };
-            // S = Q[i] . K tile j; the last query tile to use the K tile frees it
-            auto mma_s = [&](int i, int j, bool frees) {
+                use++;
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
-                    const int gg = k_stage(j) + part;
-                    wait(&full[gg % NST], (gg / NST) & 1);
-                    if (!ok) return;
-                    const uint32_t kb = smem_u32(ring + (gg % NST) * C::STAGE);
-                    const uint32_t qb = smem_u32(qs + i * C::QTILE) + part * (C::SPAN / 64) * pa::PANEL;
+                    const int gg = (j == 0 ? 0 : 2 * j - 1) * PARTS + part;
+                    if (first) wait(&full[gg % NST], (gg / NST) & 1);
+                    if (!ok) break;
+                    const uint32_t kb = smem_u32(ring) + (gg % NST) * C::STAGE;
+                    const uint32_t qb = smem_u32(qs) + i * C::QTILE + part * (C::SPAN / 64) * pa::PANEL;
 #pragma unroll
                     for (int k = 0; k < C::SPAN / 16; k++) {
                         const uint32_t off = (k >> 2) * pa::PANEL + (k & 3) * 32;
                         tc_mma_warp(tmem, umma_desc_sw128(qb + off), umma_desc_sw128(kb + off), C::IDESC_S, (part | k) != 0);
                     }
-                    if (frees) tc_commit_warp(&empty[gg % NST]);
+                    if (last) tc_commit_warp(&empty[gg % NST]);
                 }
-                tc_commit_warp(&s_full[i]);
-            };
-            // O[i] (+)= P[i] . V tile j
-            auto mma_o = [&](int i, int j, bool frees) {
+                if (ok) tc_commit_warp(&s_full[i]);
+            }
+    } else if (warp == 3) {             // ---- O += P . V
+        const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
+        const int mf = __shfl_sync(0xffffffffu, mask_from, 0), n = max(n0, n1);
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, int parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
+        };
+        for (int j = 0; j < n && ok; j++)
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                if (!ok || j >= (i == 0 ? n0 : n1)) continue;
+                const bool first = i == 0 || j >= n0, last = i == NQ - 1 || j >= n1;   // to use this V tile
+                wait(&p_full[p_at(i, j)], p_use(j) & 1);
+                tc_fence_after();
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
-                    const int gg = v_stage(j) + part;
-                    wait(&full[gg % NST], (gg / NST) & 1);
-                    if (j >= mf) wait(&checked[gg % NST], (gg / NST) & 1);
-                    if (!ok) return;
-                    const uint32_t vb = smem_u32(ring + (gg % NST) * C::STAGE);
+                    const int gg = (j == n - 1 ? 2 * n - 1 : 2 * j + 2) * PARTS + part;
+                    if (first) wait(&full[gg % NST], (gg / NST) & 1);
+                    if (first && j >= mf) wait(&checked[gg % NST], (gg / NST) & 1);
+                    if (!ok) break;
+                    const uint32_t vb = smem_u32(ring) + (gg % NST) * C::STAGE;
 #pragma unroll
                     for (int k = 0; k < pa::BN / 16; k++)
-                        tc_mma_ts_warp(tmem + C::O_COL + i * D + part * C::SPAN, tmem + C::P_COL + i * 64 + k * 8,
-                                       umma_desc_mn_sw128(vb + k * 2048, pa::PANEL), C::IDESC_O, j > 0 || k != 0);
-                    if (frees) tc_commit_warp(&empty[gg % NST]);
+                        tc_mma_ts_warp(tmem + C::O_COL + i * D + part * C::SPAN, tmem + C::P_COL + p_at(i, j) * 64 + k * 8,
+                                       umma_desc_mn_sw128(vb + k * 2048, pa::PANEL), C::IDESC_O, k ? 1u : (uint32_t)(j > 0));
+                    if (last) tc_commit_warp(&empty[gg % NST]);
                 }
-                tc_commit_warp(&o_done[i]);
-            };
-            // The uses of S: tile j of query tile 0, of query tile 1 (while they have
-            // tiles left), then j + 1.  S is free again as soon as the softmax has it
-            // in registers, so the products of S run NQ + 1 uses ahead of those of O:
-            // the softmax that ends finds its next S there.
-            int si = n0 > 0 ? 0 : 1, sj = 0, su = 0;
-            auto next_s = [&]() {
-                if (su >= total) return;
-                if (su > 0) wait(&s_free, (su - 1) & 1);
-                if (!ok) return;
-                const bool more = si == 0 && sj < n1;       // query tile 1 follows with the same K tile
-                mma_s(si, sj, !more);
-                if (more) si = 1;
-                else { sj++; si = sj < n0 ? 0 : 1; }
-                su++;
-            };
-            wait(&q_full, 0);
-            for (int k = 0; k <= NQ && ok; k++) next_s();
-            for (int j = 0; j < ntmax && ok; j++)
-                for (int i = 0; i < NQ && ok; i++) {
-                    if (j >= (i == 0 ? n0 : n1)) continue;
-                    wait(&p_full[i], j & 1);
-                    if (!ok) break;
-                    mma_o(i, j, i == 1 || j >= n1);
-                    if (ok) next_s();
-                }
-        }
-    } else if (warp < 4) {              // ---- V tiles with hidden keys
-        const int w64 = tid - 64;
+                if (ok) tc_commit_warp(&o_done[p_at(i, j)]);
+            }
+    } else if (warp == 2) {             // ---- V tiles with hidden keys
         int g = 0;
         bool ok = true;
         for (int e = 0; e < entries && ok; e++) {
@@ -302,16 +296,16 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                     const int behind = sq.m - tile * pa::BN;        // rows from here on belong to no key
                     // eight 16-byte pieces at a time: an exponent of all ones carries
                     // into the sign bit
-                    for (int i = w64 * 16; i < C::STAGE; i += 8 * 64 * 16) {
+                    for (int i = lane * 16; i < C::STAGE; i += 8 * 32 * 16) {
                         uint4 w[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) w[k] = lds128(st + i + k * 1024);
+                        for (int k = 0; k < 8; k++) w[k] = lds128(st + i + k * 512);
                         if (behind < pa::BN) {
 #pragma unroll
                             for (int k = 0; k < 8; k++)
-                                if ((((i + k * 1024) / 128) & 127) >= behind) {
+                                if ((((i + k * 512) / 128) & 127) >= behind) {
                                     w[k] = make_uint4(0, 0, 0, 0);
-                                    *(uint4 *)(st + i + k * 1024) = w[k];
+                                    *(uint4 *)(st + i + k * 512) = w[k];
                                 }
                         }
                         uint32_t bad = 0;
@@ -322,7 +316,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                         if (!(bad & 0x80008000u)) continue;
 #pragma unroll 1
                         for (int k = 0; k < 8; k++) {
-                            const int at = i + k * 1024, r = (at / 128) & 127;
+                            const int at = i + k * 512, r = (at / 128) & 127;
                             // the piece's place in its row is swizzled by the row
                             const int d0 = part * C::SPAN + (at / pa::PANEL) * 64 + (((at >> 4) & 7) ^ (r & 7)) * 8;
                             uint16_t *h = (uint16_t *)(st + at);
@@ -342,7 +336,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                             }
                         }
                     }
-                    static_assert(C::STAGE % (8 * 64 * 16) == 0, "whole batches of pieces");
+                    static_assert(C::STAGE % (8 * 32 * 16) == 0, "whole batches of pieces");
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
                 __syncwarp();
@@ -358,7 +352,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
         const int rt = (warp & 3) * 32 + lane, row = r0 + i * pa::BM + rt;      // row in the sequence
         const int nti = nt[i];
         const int seen = max(0, min(sq.m, sq.m - sq.n + min(row, sq.n - 1) + 1));   // keys that it sees
-        const uint32_t p_col = tmem + lanes + C::P_COL + i * 64, o_col = tmem + lanes + C::O_COL + i * D;
+        const uint32_t o_col = tmem + lanes + C::O_COL + i * D;
         float m = -INFINITY, l = 0.f;
         const float raise = pa::RAISE / a.zscale;
         bool ok = true;
@@ -386,12 +380,17 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], v[c + u]);
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool up = top > m + raise;
-            // P's place is read by the product of j - 1 until that is done
-            if (j > 0) {
-                wait(&o_done[i], (j - 1) & 1);
+            // P's place is read by the product of j - 1 (NQ 1: j - 2) until that is done
+            const uint32_t p_col = tmem + lanes + C::P_COL + p_at(i, j) * 64;
+            if (j >= (NQ == 2 ? 1 : 2)) {
+                wait(&o_done[p_at(i, j)], (p_use(j) - 1) & 1);
                 if (!ok) break;
             }
             if (__any_sync(0xffffffffu, up)) {
+                if (NQ == 1 && j > 0) {      // O is the product's of j - 1 until that is done
+                    wait(&o_done[p_at(i, j - 1)], p_use(j - 1) & 1);
+                    if (!ok) break;
+                }
                 const float down = !up ? 1.0f : m == -INFINITY ? 0.f : pa_ex2((m - top) * a.zscale);
                 if (up) m = top;
                 l *= down;
@@ -423,9 +422,10 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_full[i]);
+            mbar_arrive(&p_full[p_at(i, j)]);
         }
-        if (ok && nti > 0) wait(&o_done[i], (nti - 1) & 1);
+        if (NQ == 1 && ok && nti > 1) wait(&o_done[p_at(i, nti - 2)], p_use(nti - 2) & 1);
+        if (ok && nti > 0) wait(&o_done[p_at(i, nti - 1)], p_use(nti - 1) & 1);
         if (ok) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             uint16_t *op = a.out.p + (long)(sq.q0 + row) * a.out.rs + (long)head * a.out.hs;
