@@ -380,21 +380,13 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], v[c + u]);
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool up = top > m + raise;
-            // P's place is read by the product of j - 1 (NQ 1: j - 2) until that is done
-            const uint32_t p_col = tmem + lanes + C::P_COL + p_at(i, j) * 64;
-            if (j >= (NQ == 2 ? 1 : 2)) {
-                wait(&o_done[p_at(i, j)], (p_use(j) - 1) & 1);
-                if (!ok) break;
-            }
             if (__any_sync(0xffffffffu, up)) {
-                if (NQ == 1 && j > 0) {      // O is the product's of j - 1 until that is done
-                    wait(&o_done[p_at(i, j - 1)], p_use(j - 1) & 1);
-                    if (!ok) break;
-                }
                 const float down = !up ? 1.0f : m == -INFINITY ? 0.f : pa_ex2((m - top) * a.zscale);
                 if (up) m = top;
                 l *= down;
-                if (j > 0) {
+                if (j > 0) {                 // O is the product's of j - 1 until that is done
+                    wait(&o_done[p_at(i, j - 1)], p_use(j - 1) & 1);
+                    if (!ok) break;
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
@@ -407,19 +399,23 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             }
             const float mz = m == -INFINITY ? 0.f : m * a.zscale;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t pk[2][32];
 #pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int u = 0; u < 32; u += 2) {
-                    const float p0 = pa_ex2(fmaf(v[c + u], a.zscale, -mz)), p1 = pa_ex2(fmaf(v[c + u + 1], a.zscale, -mz));
-                    sum[u & 2] += p0;
-                    sum[(u & 2) + 1] += p1;
-                    pk[u / 2] = pa_pack(p0, p1);
-                }
-                tc_st16(p_col + c / 2, pk);
+            for (int c = 0; c < 128; c += 2) {
+                const float p0 = pa_ex2(fmaf(v[c], a.zscale, -mz)), p1 = pa_ex2(fmaf(v[c + 1], a.zscale, -mz));
+                sum[c & 2] += p0;
+                sum[(c & 2) + 1] += p1;
+                pk[c / 64][(c % 64) / 2] = pa_pack(p0, p1);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            // P's place is read by the product of j - 1 (NQ 1: j - 2) until that is done
+            if (j >= (NQ == 2 ? 1 : 2)) {
+                wait(&o_done[p_at(i, j)], (p_use(j) - 1) & 1);
+                if (!ok) break;
+            }
+            const uint32_t p_col = tmem + lanes + C::P_COL + p_at(i, j) * 64;
+            tc_st32(p_col, pk[0]);
+            tc_st32(p_col + 32, pk[1]);
             tc_wait_st();
             tc_fence_before();
             mbar_arrive(&p_full[p_at(i, j)]);
