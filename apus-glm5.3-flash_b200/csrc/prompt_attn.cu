@@ -17,7 +17,9 @@
 // Up to dim 128 two query tiles share an SM, so that each K and V tile serves 256
 // rows and one tile's softmax runs under the other's products.  S has one place
 // in TMEM, which the softmax frees as soon as it holds the scores in registers; P
-// has a place of its own.  So the next S is there when a softmax ends.  (With P
+// has a place of its own.  So the next S is there when a softmax ends, and the two
+// softmaxes take turns at the exponentials (at dim 64, with an S place each, they
+// ran in step and took 10% longer).  (With P
 // written over S, a query tile waited 1400 of 3700 cycles for its own products;
 // two S tiles of 64 keys made the products of S, which read 128 rows of Q for 64
 // keys, the bound.)
@@ -33,8 +35,6 @@
 // (and all rows behind the sequence) are set to 0 in shared memory before the
 // product reads them; the first key with a NaN, a +inf and a -inf is kept for each
 // dim, and the rows that see it get it added at the end.
-#include <type_traits>
-
 #include "attn_dev.h"
 #include "common.cuh"
 #include "pipe.cuh"
@@ -74,7 +74,7 @@ template <int D> struct Cfg {
     static constexpr int NST = D == 256 ? 5 : D == 128 ? 4 : 8;
     static constexpr int SMEM = NQ * QTILE + NST * STAGE + 1024;
     static constexpr int ROWS = NQ * BM;
-    static constexpr int P_COL = 128, O_COL = 256;          // TMEM: S from 0, two P, each query tile's O
+    static constexpr int P_COL = 128, O_COL = 256;          // TMEM columns: S from 0, P (two places), O
     // D f32, A and B BF16, N >> 3 at bit 17, M >> 4 at bit 24; V has its dims
     // (N) contiguous: bit 16
     static constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) |
@@ -103,7 +103,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     using C = pa::Cfg<D>;
     constexpr int NQ = C::NQ, NST = C::NST, PARTS = C::PARTS;
     extern __shared__ __align__(1024) uint8_t pa_dyn[];
-    __shared__ __align__(8) uint64_t q_full, full[NST], empty[NST], checked[NST], s_free, s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(8) uint64_t q_full[PARTS], full[NST], empty[NST], checked[NST], s_free, s_full[2], p_full[2], o_done[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, poison, found_s[2], wsum[C::THREADS / 32];
     // first key (from the first looked after, 1023: none) with a NaN, +inf, -inf in
@@ -117,6 +117,21 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     // with the most keys) first
     const int head = (int)(blockIdx.x % (unsigned)a.heads), block = (int)(blockIdx.x / (unsigned)a.heads);
     if (tid == 0) found_s[0] = -1;
+    for (int i = tid; i < D; i += C::THREADS) first_bad[i] = 0x3fffffffu;
+    if (tid == 0) {
+        for (int p = 0; p < PARTS; p++) mbar_init(&q_full[p], 1);
+        for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&checked[s], 1); }   // empty: products, scan
+        mbar_init(&s_free, 128);
+        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_done[i], 1); }
+        abort_flag = 0;
+        poison = 0;
+        fence_barrier_init();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     {
         int before = 0;
         for (int s0 = 0; s0 < a.nseq && before <= block; s0 += C::THREADS) {
@@ -139,7 +154,14 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             __syncthreads();
         }
     }
-    if (found_s[0] < 0) return;
+    if (found_s[0] < 0) {
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (warp == 2)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(512) : "memory");
+        return;
+    }
     const PromptSeq sq = prompt_seq(a, found_s[0], false);
     const int r0 = found_s[1] * C::ROWS;                    // first row of the block, in the sequence
     const int khead = head / a.group;
@@ -157,21 +179,6 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     }
     const int ntmax = max(nt[0], nt[1]);
 
-    for (int i = tid; i < D; i += C::THREADS) first_bad[i] = 0x3fffffffu;
-    if (tid == 0) {
-        mbar_init(&q_full, 1);
-        for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&checked[s], 1); }   // empty: products, scan
-        mbar_init(&s_free, 128);
-        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_done[i], 1); }
-        abort_flag = 0;
-        poison = 0;
-        fence_barrier_init();
-    }
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -193,10 +200,6 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     };
     if (warp == 0) {
         if (lane == 0 && ntmax > 0) {   // ---- copies
-            mbar_arrive_expect_tx(&q_full, NQ * C::QTILE);
-            for (int i = 0; i < NQ; i++)
-                for (int p = 0; p < D / 64; p++)
-                    tma_load_3d(qs + i * C::QTILE + p * pa::PANEL, &qmap, p * 64, head, sq.q0 + r0 + i * pa::BM, &q_full);
             int g = 0;
             bool ok = true;
             for (int e = 0; e < entries && ok; e++) {
@@ -205,6 +208,13 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 entry(e, is_v, tile);
                 for (int part = 0; part < PARTS && ok; part++, g++) {
                     const int s = g % NST;
+                    if (e == 0) {       // this part of Q, then of the first K: the first product can begin
+                        mbar_arrive_expect_tx(&q_full[part], NQ * C::STAGE);
+                        for (int i = 0; i < NQ; i++)
+                            for (int p = part * (C::SPAN / 64); p < (part + 1) * (C::SPAN / 64); p++)
+                                tma_load_3d(qs + i * C::QTILE + p * pa::PANEL, &qmap, p * 64, head,
+                                            sq.q0 + r0 + i * pa::BM, &q_full[part]);
+                    }
                     if (g >= NST && !(ok = mbar_wait(&empty[s], ((g / NST) - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT))) break;
                     mbar_arrive_expect_tx(&full[s], C::STAGE);
                     for (int p = 0; p < C::SPAN / 64; p++)
@@ -220,7 +230,6 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
                 ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
         };
-        if (ntmax > 0) wait(&q_full, 0);
         // The uses of S: key tile j of query tile 0, then of query tile 1, while they
         // have tiles left.  S is free again as soon as a softmax has it in registers,
         // so the softmax that ends finds its next S there.
@@ -236,6 +245,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
                     const int gg = (j == 0 ? 0 : 2 * j - 1) * PARTS + part;
+                    if (use == 1) wait(&q_full[part], 0);
                     if (first) wait(&full[gg % NST], (gg / NST) & 1);
                     if (!ok) break;
                     const uint32_t kb = smem_u32(ring) + (gg % NST) * C::STAGE;
@@ -422,9 +432,14 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
         }
         if (NQ == 1 && ok && nti > 1) wait(&o_done[p_at(i, nti - 2)], p_use(nti - 2) & 1);
         if (ok && nti > 0) wait(&o_done[p_at(i, nti - 1)], p_use(nti - 1) & 1);
+        // a query tile that sees no key: its rows of Q may still be on their way
+        if (nti == 0 && ntmax > 0)
+            for (int p = 0; p < PARTS; p++) wait(&q_full[p], 0);
         if (ok) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            uint16_t *op = a.out.p + (long)(sq.q0 + row) * a.out.rs + (long)head * a.out.hs;
+            // through this warp's rows of the Q tile, which nothing reads any more, so
+            // that rows are stored whole: 16-byte pieces, swizzled by the row
+            uint8_t *own = qs + i * C::QTILE + (warp & 3) * 32 * (D * 2);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
@@ -441,17 +456,25 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                         o[u] = __float_as_uint(x);
                     }
                 }
-                if (row < sq.n) {
 #pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        uint32_t w[4];
+                for (int h = 0; h < 4; h++) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            w[u] = nti > 0 ? pa_pack(__uint_as_float(o[8 * h + 2 * u]) * inv,
-                                                     __uint_as_float(o[8 * h + 2 * u + 1]) * inv) : 0u;
-                        *(uint4 *)(op + c + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int u = 0; u < 4; u++)
+                        w[u] = nti > 0 ? pa_pack(__uint_as_float(o[8 * h + 2 * u]) * inv,
+                                                 __uint_as_float(o[8 * h + 2 * u + 1]) * inv) : 0u;
+                    *(uint4 *)(own + lane * (D * 2) + (((c / 8 + h) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+            }
+            __syncwarp();
+            constexpr int PIECES = D / 8, RPS = 32 / PIECES > 0 ? 32 / PIECES : 1;     // pieces of a row, rows of a store
+            const int left = sq.n - (row - lane);                                      // rows of this warp that exist
+#pragma unroll 4
+            for (int r = 0; r < 32; r += RPS) {
+                const int rr = r + (RPS > 1 ? lane / PIECES : 0), p = RPS > 1 ? lane % PIECES : lane;
+                if (rr < left)
+                    *(uint4 *)(a.out.p + (long)(sq.q0 + row - lane + rr) * a.out.rs + (long)head * a.out.hs + p * 8) =
+                        lds128(own + rr * (D * 2) + ((p ^ (rr & 7)) << 4));
             }
         }
     }
