@@ -235,26 +235,38 @@ apus_gcuda_prompt_attn_dev = _fn("apus_gcuda_prompt_attn_dev", _i, _pb_p, _rows_
                                  _f, _vp)
 
 
-def _same_device(what, dev, *tensors):
-    """Every tensor on the CUDA device `dev`, and that the current one."""
-    import torch
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise GcudaError(f"{what}: tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise GcudaError(f"{what}: tensors on {dev}, not on a GPU")
-    if dev.index != torch.cuda.current_device():
-        raise GcudaError(f"{what}: tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
-
-
 def head_rows(t, what="rows"):
     """ApusHeadRows of a BF16 tensor [rows][heads][dim] (strided views too, the
     dims contiguous)."""
     import torch
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise GcudaError(f"{what}: BF16 [rows][heads][dim] with contiguous dims, not {t.dtype} {list(t.shape)} "
+    shape = t.shape
+    if len(shape) != 3 or t.dtype is not torch.bfloat16 or (shape[2] > 1 and t.stride(2) != 1):
+        raise GcudaError(f"{what}: BF16 [rows][heads][dim] with contiguous dims, not {t.dtype} {list(shape)} "
                          f"with strides {t.stride()}")
-    return HeadRows(t.data_ptr(), t.shape[0], t.shape[1], t.stride(0), t.stride(1))
+    s = t.stride()
+    return HeadRows(t.data_ptr(), shape[0], shape[1], s[0], s[1])
+
+
+def _on(what, index, *tensors):
+    """Every tensor on GPU `index`, and that the current device.  Called for
+    every operator call: plain integers, no torch.device objects."""
+    import torch
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise GcudaError(f"{what}: a tensor on {t.device}, others on "
+                             f"{'cuda:%d' % index if index >= 0 else 'the host'}")
+    if index < 0:
+        raise GcudaError(f"{what}: tensors on the host, not on a GPU")
+    if index != torch.cuda.current_device():
+        raise GcudaError(f"{what}: tensors on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _raw_stream(index, stream):
+    """The CUDA stream handle of a torch stream, or of the current one."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _ints(what, t, dim):
@@ -273,6 +285,7 @@ class Kv4Cache:
             raise GcudaError(f"kv4 cache: contiguous uint8 [pages][heads][72 * dim], not {pages.dtype} "
                              f"{list(pages.shape)}")
         self.pages, self.heads, self.dim = pages, pages.shape[1], pages.shape[2] // 72
+        self.index = pages.get_device()
         self.desc = Kv4CacheDesc(pages.data_ptr(), pages.shape[0], self.heads, self.dim)
         self.ref = C.pointer(self.desc)
 
@@ -298,7 +311,9 @@ class Kv4Batch:
         n = kv_len.shape[0]
         if cu_rows.shape[0] != n + 1 or page_table.shape[0] != n:
             raise GcudaError(f"kv4 batch: {n} sequences, {cu_rows.shape[0]} row starts, {page_table.shape[0]} page lists")
-        self.tensors = (cu_rows, kv_len, page_table)
+        self.tensors, self.index = (cu_rows, kv_len, page_table), kv_len.get_device()
+        if cu_rows.get_device() != self.index or page_table.get_device() != self.index:
+            raise GcudaError(f"kv4 batch: tensors on {cu_rows.device}, {kv_len.device} and {page_table.device}")
         self.desc = Kv4BatchDesc(cu_rows.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
                                  page_table.stride(0) if n > 1 else page_table.shape[1], n, max_rows, max_len)
         self.ref = C.pointer(self.desc)
@@ -313,30 +328,33 @@ class PromptBatch:
         _ints("cu_k", cu_k, 1)
         if cu_q.shape != cu_k.shape or cu_q.shape[0] < 1:
             raise GcudaError(f"prompt batch: {cu_q.shape[0]} and {cu_k.shape[0]} row starts")
-        self.tensors = (cu_q, cu_k)
+        self.tensors, self.index = (cu_q, cu_k), cu_q.get_device()
+        if cu_k.get_device() != self.index:
+            raise GcudaError(f"prompt batch: tensors on {cu_q.device} and {cu_k.device}")
         self.desc = PromptBatchDesc(cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, max_rows)
         self.ref = C.pointer(self.desc)
 
 
-def _kv4_call(what, cache, batch, dim_of, *more):
-    for t in dim_of:
-        if t.shape[-1] != cache.dim:
-            raise GcudaError(f"{what}: head dim {t.shape[-1]}, the cache's is {cache.dim}")
-    _same_device(what, cache.pages.device, *batch.tensors, *dim_of, *more)
+def _kv4_call(what, cache, batch, x, y, *more):
+    if x.shape[-1] != cache.dim or y.shape[-1] != cache.dim:
+        raise GcudaError(f"{what}: head dims {x.shape[-1]}, {y.shape[-1]}, the cache's is {cache.dim}")
+    if batch.index != cache.index:
+        raise GcudaError(f"{what}: cache and batch on different devices")
+    _on(what, cache.index, x, y, *more)
 
 
 def kv4_append(cache, batch, k, v, stream=None):
     """Quantise the batch's rows k, v [rows][heads][dim] into the cache."""
-    _kv4_call("kv4_append", cache, batch, (k, v))
-    check(apus_gcuda_kv4_append_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"), stream_of(stream)),
-          "kv4_append")
+    _kv4_call("kv4_append", cache, batch, k, v)
+    check(apus_gcuda_kv4_append_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"),
+                                    _raw_stream(cache.index, stream)), "kv4_append")
 
 
 def kv4_read(cache, batch, k, v, stream=None):
     """Read the batch's rows back into k, v [rows][heads][dim]."""
-    _kv4_call("kv4_read", cache, batch, (k, v))
-    check(apus_gcuda_kv4_read_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"), stream_of(stream)),
-          "kv4_read")
+    _kv4_call("kv4_read", cache, batch, k, v)
+    check(apus_gcuda_kv4_read_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"),
+                                  _raw_stream(cache.index, stream)), "kv4_read")
 
 
 def kv4_attn_workspace(cache, batch, q_heads):
@@ -352,7 +370,7 @@ def kv4_attn(cache, batch, q, out, scale, workspace=None, sel=None, pool=0, stre
     """Attention of q [rows][q_heads][dim] over the cache into out; sel: uint8
     [rows][pools], the pools of `pool` positions that each row keeps."""
     import torch
-    _kv4_call("kv4_attn", cache, batch, (q, out), workspace, sel)
+    _kv4_call("kv4_attn", cache, batch, q, out, workspace, sel)
     if sel is not None and (sel.dtype != torch.uint8 or sel.dim() != 2 or sel.shape[0] < q.shape[0] or
                             not sel.is_contiguous()):
         raise GcudaError(f"kv4_attn: sel is contiguous uint8 [rows][pools], not {sel.dtype} {list(sel.shape)}")
@@ -361,17 +379,18 @@ def kv4_attn(cache, batch, q, out, scale, workspace=None, sel=None, pool=0, stre
                                   0 if sel is None else sel.shape[1], pool,
                                   None if workspace is None else workspace.data_ptr(),
                                   0 if workspace is None else workspace.numel() * workspace.element_size(),
-                                  stream_of(stream)), "kv4_attn")
+                                  _raw_stream(cache.index, stream)), "kv4_attn")
 
 
 def prompt_attn(batch, q, k, v, out, scale, stream=None):
     """Causal attention over packed prompts: q, out [rows][q_heads][dim],
     k, v [keys][heads][dim]."""
-    if not q.shape[-1] == k.shape[-1] == v.shape[-1] == out.shape[-1]:
+    dim = q.shape[-1]
+    if k.shape[-1] != dim or v.shape[-1] != dim or out.shape[-1] != dim:
         raise GcudaError(f"prompt_attn: head dims {[t.shape[-1] for t in (q, k, v, out)]}")
-    _same_device("prompt_attn", q.device, k, v, out, *batch.tensors)
+    _on("prompt_attn", batch.index, q, k, v, out)
     check(apus_gcuda_prompt_attn_dev(batch.ref, head_rows(q, "q"), head_rows(k, "k"), head_rows(v, "v"),
-                                     head_rows(out, "out"), q.shape[-1], scale, stream_of(stream)), "prompt_attn")
+                                     head_rows(out, "out"), dim, scale, _raw_stream(batch.index, stream)), "prompt_attn")
 
 
 EP_HANDLE_BYTES = 64   # sizeof(cudaIpcMemHandle_t)
