@@ -70,10 +70,14 @@ template <int D> struct Cfg {
     // pairs of positions, and each position's power of two with its inverse
     static constexpr int KF = STAGES * STAGE, VH = KF + U * NG * 4, PW = VH + U * NG * 2;
     static constexpr int WARP_SMEM = PW + U * 8;
-    static constexpr int SMEM = WARPS * WARP_SMEM;
-    static constexpr int LIST = 2048;                       // selected positions at a time (16-bit offsets)
+    // the query's fragments, 512 bytes a group: 32 registers at dim 256, which the
+    // loop has not (it spilt); below they stay in registers
+    static constexpr bool QS = D == 256;
+    static constexpr int QF = WARPS * WARP_SMEM, SMEM = QF + (QS ? NG * 512 : 0);
 };
-constexpr int LIST_SPAN = 32768;                            // positions that one list can cover
+// Selected positions at a time: an offset in bits 0-15, above them a bit for
+// each row of the block that keeps the position.
+constexpr int LIST = 4096, LIST_SPAN = 65536, LOOK = 4;     // LOOK: pools that a thread looks at together
 constexpr float NEG_INF = -__builtin_huge_valf();
 }  // namespace kv4
 
@@ -98,6 +102,8 @@ APUS_DEV long div_long(long a, long b) {
     return ((unsigned long)(a | b) >> 32) == 0 ? (long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 APUS_DEV int row_of(const Kv4AttnArgs &a, int c) { return (int)(((uint64_t)(uint32_t)c * a.group_magic) >> 40); }
+
+APUS_DEV int pool_of(const Kv4AttnArgs &a, int j) { return (int)(((uint64_t)(uint32_t)j * a.pool_magic) >> 36); }
 
 constexpr int KJ_RUNS = 148 * 4;          // runs at most (a multiple of 4)
 
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     int seq = (int)found_s[0];
     long seq_x = found_s[1];
     uint8_t *const own = kv4_dyn + warp * C::WARP_SMEM, *const stages = own;
-    uint16_t *list = (uint16_t *)(kv4_dyn + C::SMEM);
+    uint32_t *list = (uint32_t *)(kv4_dyn + C::SMEM);     // LIST entries and 16 that no row keeps
     __shared__ int wcount[kv4::WARPS];
 
     while (x < xe) {
@@ -293,16 +299,20 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
 
     // the query rows of this lane's columns, on their way while the first units are fetched
     uint4 raw[NT][NG];
+    auto fetch_query = [&]() {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int c = c0 + nt * 8 + g, t = row_of(a, min(c, cols - 1));
-        const uint16_t *qp = a.q.p + (long)(sq.row0 + t) * a.q.rs + (long)(head * a.group + min(c, cols - 1) - t * a.group) * a.q.hs;
+        for (int nt = 0; nt < NT; nt++) {
+            const int c = c0 + nt * 8 + g, t = row_of(a, min(c, cols - 1));
+            const uint16_t *qp = a.q.p + (long)(sq.row0 + t) * a.q.rs + (long)(head * a.group + min(c, cols - 1) - t * a.group) * a.q.hs;
 #pragma unroll
-        for (int j = 0; j < NG; j++)
-            raw[nt][j] = c < cols ? *(const uint4 *)(qp + 32 * j + 8 * q4) : make_uint4(0, 0, 0, 0);
-    }
-    // the query's fragments, the columns' offsets, factors and limits (below)
-    uint32_t Q[NT][NG][4];
+            for (int j = 0; j < NG; j++)
+                raw[nt][j] = c < cols ? *(const uint4 *)(qp + 32 * j + 8 * q4) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (!SEL) fetch_query();
+    // the query's fragments, the columns' offsets, factors and limits (SEL: the
+    // bit of the column's row in a list entry; below)
+    uint32_t Q[C::QS ? 1 : NT][C::QS ? 1 : NG][4];
     float cinit[NT][NG][2], fac[NT][2];
     int lim[NT][2];
     float O[NT][D / 16][4], m[NT][2], l[NT][2];      // columns 2 q4, 2 q4 + 1; l: this lane's positions
@@ -359,8 +369,8 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     };
 
     // 16 positions at place `at` of a stage: the positions from pos0 on, or (SEL)
-    // those that the list names, n of them
-    auto process = [&](const uint8_t *st, int at, int pos0, const uint16_t *names, int n, auto masked_t) {
+    // those that the list names
+    auto process = [&](const uint8_t *st, int at, int pos0, const uint32_t *names, auto masked_t) {
         constexpr bool MASKED = decltype(masked_t)::value;
         float z[NT][4];                // positions pg (0, 1), pg + 8 (2, 3); columns 2 q4 (0, 2), 2 q4 + 1
         float2 pw[2];                  // their powers of two
@@ -387,10 +397,11 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_f16(c, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u,
-                            Q[nt][j][0], Q[nt][j][1]);
-                    mma_f16(c, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, Q[nt][j][2],
-                            Q[nt][j][3]);
+                    uint4 qf;
+                    if constexpr (C::QS) qf = lds128(kv4_dyn + C::QF + j * 512 + lane * 16);
+                    else qf = make_uint4(Q[nt][j][0], Q[nt][j][1], Q[nt][j][2], Q[nt][j][3]);
+                    mma_f16(c, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, qf.x, qf.y);
+                    mma_f16(c, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, qf.z, qf.w);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float x = c[i] + cinit[nt][j][i & 1], s = i < 2 ? sa[j] : sb[j];
@@ -407,28 +418,16 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         uint32_t hide = 0;             // bit nt * 4 + i (MASKED)
         bool over = false;
         float high[NT][2];
+        uint32_t name[2] = {0, 0};
+        if (SEL) { name[0] = names[pg]; name[1] = names[pg + 8]; }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            int tail[2] = {0, 0};      // where a column's incomplete pool begins
-            const uint8_t *srow[2] = {nullptr, nullptr};
-            if (SEL) {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    tail[u] = lim[nt][u] > 0 ? lim[nt][u] - lim[nt][u] % a.pool : 0;
-                    srow[u] = a.sel + (long)(sq.row0 + lim[nt][u] - lim_row0) * a.sel_stride;
-                }
-            }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float v = fmaf(z[nt][i], fac[nt][i & 1], pw[i >> 1].x);
                 if (MASKED) {
-                    const int o = (i >> 1) * 8 + pg;
-                    const int j = SEL ? (o < n && names[o] != 0xffff ? pos0 + names[o] : 0x7fffffff) : pos0 + o;
-                    bool see = j < lim[nt][i & 1];
-                    if (SEL && see && j < tail[i & 1]) {
-                        const long pl = (long)(((uint64_t)(uint32_t)j * a.pool_magic) >> 36);
-                        see = pl < a.sel_stride && srow[i & 1][pl] != 0;
-                    }
+                    const bool see = SEL ? (name[i >> 1] >> lim[nt][i & 1] & 1) != 0
+                                         : pos0 + (i >> 1) * 8 + pg < lim[nt][i & 1];
                     if (!see) { v = NEG_INF; hide |= 1u << (nt * 4 + i); }
                 }
                 z[nt][i] = v;
@@ -509,28 +508,46 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     do {
         int base = p0, filled = p1 > p0 ? p1 - p0 : 0;     // positions, the first of them (SEL: of the list)
         if constexpr (SEL) {
-            // list the positions from `done` on that a row keeps, as many as the
-            // list holds: a thread looks at one pool
+            // list the positions from `done` on that a row keeps, as many as the list
+            // holds.  Pools are whole but for the first, which the piece's begin may
+            // cut, and the last; a row sees all of its own incomplete pool.
             __syncthreads();
-            const int t0 = lim0 - lim_row0, t1 = lim1 - lim_row0;          // rows of the block
+            const int t0 = lim0 - lim_row0, nt = lim1 - lim0 + 1;          // rows of the block
+            const uint8_t *const sel0 = a.sel + (long)(sq.row0 + t0) * a.sel_stride;
             const int span = min(p1, done + kv4::LIST_SPAN);
             base = done;
             filled = 0;
-            // pools looked at together: one at least (a pool has at most 128
-            // positions, the list room for 2048), so `done` advances each time
-            const int round = min(kv4::THREADS, C::LIST / a.pool);
-            while (done < span && filled + round * a.pool <= C::LIST) {
-                const int pl = done / a.pool + (int)threadIdx.x;
-                const int b = max(pl * a.pool, done), e = min((pl + 1) * a.pool, span);
-                bool any = false;
-                if ((int)threadIdx.x < round && b < e)
-                    for (int t = t0; t <= t1; t++) {
-                        const int lim = lim_row0 + t;
-                        if (lim <= b) continue;
-                        any |= b >= lim - lim % a.pool ||
-                               (pl < a.sel_stride && a.sel[(long)(sq.row0 + t) * a.sel_stride + pl] != 0);
+            // pools looked at together: at least one, with room in the list for twice as
+            // many positions, so `done` advances each time
+            const int round = min(kv4::THREADS * kv4::LOOK, kv4::LIST / 2 / a.pool);
+            const int tail0 = lim0 > 0 ? pool_of(a, lim0) * a.pool : 0;      // where the first row's incomplete pool begins
+            while (done < span && filled + round * a.pool <= kv4::LIST) {
+                const int pl0 = pool_of(a, done);
+                uint32_t rows[kv4::LOOK] = {};
+                for (int t = 0; t < nt; t++) {
+#pragma unroll
+                    for (int k = 0; k < kv4::LOOK; k++) {
+                        const int pl = pl0 + k * kv4::THREADS + (int)threadIdx.x;
+                        if (pl - pl0 < round && pl < a.sel_stride && pl * a.pool < span && sel0[(long)t * a.sel_stride + pl])
+                            rows[k] |= 1u << t;
                     }
-                const int cnt = any ? e - b : 0;
+                }
+                int cnt = 0, b[kv4::LOOK], n[kv4::LOOK];
+#pragma unroll
+                for (int k = 0; k < kv4::LOOK; k++) {
+                    const int at = k * kv4::THREADS + (int)threadIdx.x, first = (pl0 + at) * a.pool;
+                    b[k] = max(first, done);
+                    n[k] = 0;
+                    if (at >= round || first >= span) continue;
+                    if (first + a.pool > tail0)            // some row's incomplete pool, or behind a row's last
+                        for (int t = 0; t < nt; t++) {
+                            const int lim = lim0 + t;
+                            if (first >= lim) rows[k] &= ~(1u << t);
+                            else if (first + a.pool > lim) rows[k] |= 1u << t;
+                        }
+                    if (rows[k]) n[k] = min(first + a.pool, span) - b[k];
+                    cnt += n[k];
+                }
                 int incl = cnt;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
@@ -541,11 +558,19 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                 __syncthreads();
                 int at = filled + incl - cnt;
                 for (int w = 0; w < warp; w++) at += wcount[w];
-                for (int i = 0; i < cnt; i++) list[at + i] = (uint16_t)(b + i - base);
+#pragma unroll
+                for (int k = 0; k < kv4::LOOK; k++)
+                    for (int i = 0; i < n[k]; i++) {
+                        // row t sees positions below lim0 + t
+                        const int j = b[k] + i, from = j < lim0 ? 0 : j - lim0 + 1;
+                        list[at++] = (uint32_t)(j - base) | (rows[k] >> from << from) << 16;
+                    }
                 for (int w = 0; w < kv4::WARPS; w++) filled += wcount[w];
-                done = min(span, (done / a.pool + round) * a.pool);
+                done = min(span, (pl0 + round) * a.pool);
                 __syncthreads();
             }
+            if (threadIdx.x < 16) list[filled + threadIdx.x] = 0;
+            __syncthreads();
         }
         const int units = (filled + U - 1) / U;
         const int mine = units > warp ? (units - warp + kv4::WARPS - 1) / kv4::WARPS : 0;
@@ -592,12 +617,12 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                         src[e] = nullptr;
                         off[e] = 0;
                         if (r < U && u0 + r < filled) {
-                            const int j = base + list[u0 + r], page = table[j / KV4_PAGE];
+                            const int j = base + (int)(list[u0 + r] & 0xffffu), page = table[j / KV4_PAGE];
                             off[e] = j & (KV4_PAGE - 1);
                             if (kv4_page_ok(page, a.v.num_pages)) src[e] = a.v.pages + kv4_block_at(page, head, a.v.heads, D);
                             else {
                                 atomicExch(&g_kv4a_err, (int)ATTN_ERR_PAGE);
-                                list[u0 + r] = 0xffff;     // unseen
+                                list[u0 + r] &= 0xffffu;   // no row sees it
                             }
                         }
                     }
@@ -631,6 +656,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         };
         for (int s = 0; s < kv4::STAGES; s++) load(s, s);
         if (!SEL || base == p0) {      // once a piece, while its first units are on their way
+            if (SEL) fetch_query();
             // ---- the query's fragments: column g of each n tile, dims in the order
             // in which a lane meets the key codes (dim 8 q4 + i of a group is code i
             // of its word)
@@ -656,14 +682,21 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                     const float x[8] = {bf16lo(raw[nt][j].x), bf16hi(raw[nt][j].x), bf16lo(raw[nt][j].y), bf16hi(raw[nt][j].y),
                                         bf16lo(raw[nt][j].z), bf16hi(raw[nt][j].z), bf16lo(raw[nt][j].w), bf16hi(raw[nt][j].w)};
                     float qs = 0.f;
+                    uint32_t frag[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         // codes in the high nibbles stand 16 times higher
                         const float down = (i & 1) ? up * 0.0625f : up;
                         const uint32_t h = pack_f16(x[i] * down, x[i + 4] * down);
-                        Q[nt][j][i] = h;
+                        frag[i] = h;
                         const float2 back = __half22float2(*(const __half2 *)&h);
                         qs += (back.x + back.y) * ((i & 1) ? 16.0f : 1.0f);
+                    }
+                    if constexpr (C::QS) {
+                        if ((j & 3) == warp) *(uint4 *)(kv4_dyn + C::QF + j * 512 + lane * 16) = make_uint4(frag[0], frag[1], frag[2], frag[3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) Q[nt][j][i] = frag[i];
                     }
                     qs += __shfl_xor_sync(0xffffffffu, qs, 1);
                     qs += __shfl_xor_sync(0xffffffffu, qs, 2);
@@ -675,8 +708,12 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * q4);
             fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * q4 + 4);
 #pragma unroll
-            for (int u = 0; u < 2; u++) lim[nt][u] = lim_row0 + row_of(a, min(c0 + nt * 8 + 2 * q4 + u, cols - 1));
+            for (int u = 0; u < 2; u++) {
+                const int t = row_of(a, min(c0 + nt * 8 + 2 * q4 + u, cols - 1));
+                lim[nt][u] = SEL ? 16 + lim_row0 + t - lim0 : lim_row0 + t;
             }
+            }
+            if (C::QS) __syncthreads();
         }
         int s = 0;
         for (int i = 0; i < mine; i++) {
@@ -688,11 +725,11 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                 prepare(st);
                 if (!SEL && p0 + u0 + U <= lim0) {
 #pragma unroll 1
-                    for (int at = 0; at < U; at += 16) process(st, at, p0 + u0 + at, nullptr, 0, std::false_type{});
+                    for (int at = 0; at < U; at += 16) process(st, at, p0 + u0 + at, nullptr, std::false_type{});
                 } else {
 #pragma unroll 1
                     for (int at = 0; at < U && u0 + at < filled; at += 16)
-                        process(st, at, SEL ? base : p0 + u0 + at, list + u0 + at, filled - u0 - at, std::true_type{});
+                        process(st, at, p0 + u0 + at, list + u0 + at, std::true_type{});
                 }
             }
             __syncwarp();
@@ -869,7 +906,7 @@ int kv4_attn_args(const char *what, const ApusKv4Cache *c, const ApusKv4Batch *b
 template <int D, int NT, bool SEL>
 int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     using C = kv4::Cfg<D>;
-    const int smem = C::SMEM + (SEL ? C::LIST * 2 : 0);
+    const int smem = C::SMEM + (SEL ? (kv4::LIST + 16) * 4 : 0);
     if (gcuda_smem_limit_once((const void *)k_kv4_attn<D, NT, SEL>, smem)) return -1;
     k_kv4_attn<D, NT, SEL><<<grid, kv4::THREADS, smem, st>>>(a);
     if (gcuda_check(cudaGetLastError(), "kv4_attn launch")) return -1;
