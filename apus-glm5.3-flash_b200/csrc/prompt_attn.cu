@@ -4,31 +4,44 @@
 // for row i of n queries over m keys of one sequence, in one pass over the keys
 // with a running maximum and sum.
 //
-// Both products run on tcgen05: a CTA takes NQ tiles of 128 query rows of one
-// head and walks the keys in tiles of 128,
+// Both products run on tcgen05: an item is NQ tiles of 128 query rows of one
+// head, and a CTA walks the keys in tiles of 128,
 //   S (TMEM, fp32) = Q (shared) . K^T (shared),   O (TMEM, fp32) += P (TMEM) . V (shared),
-// with P = 2^(scale log2(e) (S - maximum)) in BF16 written over S.  K and V come as
-// tensor copies (128-byte swizzle) into a ring; V is read as it lies, rows of
-// keys with the dims contiguous.
+// with P = 2^(scale log2(e) (S - maximum)) in BF16.  K and V come as tensor copies
+// (128-byte swizzle) into a ring; V is read as it lies, rows of keys with the dims
+// contiguous.
 //
 // Bound: at dim 256 the products (2048 tensor cycles a tile of 128 x 128), at
 // dim 128 products and exponentials alike (1024 tensor cycles; 16384
 // exponentials at 16 a cycle), at dim 64 the exponentials.
-// Up to dim 128 two query tiles share an SM, so that each K and V tile serves 256
+// Up to dim 128 an item has two query tiles, so that each K and V tile serves 256
 // rows and one tile's softmax runs under the other's products.  S has one place
 // in TMEM, which the softmax frees as soon as it holds the scores in registers; P
 // has a place of its own.  So the next S is there when a softmax ends, and the two
 // softmaxes take turns at the exponentials (at dim 64, with an S place each, they
-// ran in step and took 10% longer).  (With P
-// written over S, a query tile waited 1400 of 3700 cycles for its own products;
-// two S tiles of 64 keys made the products of S, which read 128 rows of Q for 64
-// keys, the bound.)
+// ran in step and took 10% longer).  (With P written over S, a query tile waited
+// 1400 of 3700 cycles for its own products; two S tiles of 64 keys made the
+// products of S, which read 128 rows of Q for 64 keys, the bound.)
 //
 // Roles: warp 0 copies, warp 1 issues the products of S, warp 3 those of O (one
 // warp for both spent 3400 cycles on issuing 2048 cycles of products), warp 2
 // looks after V tiles with keys that some row must not see, warps 4.. are one
-// softmax group of 128 threads (a row each) a query tile.  The maximum is raised, and O rescaled, only
-// when a score passes it by more than 2^8, so almost never.
+// softmax group of 128 threads (a row each) a query tile.  The maximum is raised,
+// and O rescaled, only when a score passes it by more than 2^8, so almost never.
+// Warps 0, 1 and 3 issue as whole warps with one elected lane: in a branch that
+// one lane takes, moving the operands to uniform registers cost more than the
+// issue (1210 against 995 TFLOP/s at dim 256 for the copies alone).
+//
+// Items: a CTA that is done asks for the item of one that has not begun
+// (clusterlaunchcontrol), so the next item's copies and first products run under
+// the last one's end.  One CTA an item spent 12.7 thousand cycles on set-up, first
+// copies and the end, where 2048 rows of dim 256 take 37 thousand: 172 -> 162 us,
+// seven ragged prompts of dim 128 81 -> 75 us, nine of dim 256 71 -> 62 us.
+//
+// Measured: dim 128, 8192 rows after 4096 keys, 32 heads over 8: 0.79 ms, 1380
+// TFLOP/s; dim 256, 8192 rows of 16 heads: 1210 TFLOP/s, there bound by the ring,
+// which holds two tiles and no more fit (five half tiles in place of four: 1250;
+// quarters, V by keys, 730; two softmax groups that take turns, 1160).
 //
 // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value would
 // reach the row through the product.  So in tiles with hidden keys such values
@@ -65,14 +78,14 @@ namespace pa {
 constexpr int BM = 128, BN = 128;               // query rows of a tile, keys of a K or V tile
 constexpr int PANEL = 128 * 128;                // bytes of 128 rows of 64 dims
 template <int D> struct Cfg {
-    static constexpr int NQ = D == 256 ? 1 : 2;             // query tiles of a CTA
+    static constexpr int NQ = D == 256 ? 1 : 2;             // query tiles of an item
     static constexpr int THREADS = 128 + 128 * NQ;
     static constexpr int SPAN = D == 256 ? 128 : D;         // dims of a ring stage
     static constexpr int PARTS = D / SPAN;                  // stages of a K or V tile
-    static constexpr int STAGE = SPAN / 64 * PANEL;
-    static constexpr int QTILE = D / 64 * PANEL;
-    static constexpr int NST = D == 256 ? 5 : D == 128 ? 4 : 8;
-    static constexpr int SMEM = NQ * QTILE + NST * STAGE + 1024;
+    static constexpr int QTILE = D / 64 * PANEL, STAGE = SPAN / 64 * PANEL;
+    static constexpr int NST = D == 64 ? 8 : 4;
+    static constexpr int OUT = 32 * 128;                    // a softmax warp's rows on their way out, 64 dims of each
+    static constexpr int SMEM = NQ * QTILE + NST * STAGE + 4 * NQ * OUT + 1024;
     static constexpr int ROWS = NQ * BM;
     static constexpr int P_COL = 128, O_COL = 256;          // TMEM columns: S from 0, P (two places), O
     // D f32, A and B BF16, N >> 3 at bit 17, M >> 4 at bit 24; V has its dims
@@ -96,6 +109,49 @@ APUS_DEV uint32_t pa_pack(float lo, float hi) {
     return d;
 }
 
+// Whole-warp forms: one elected lane acts, the operands stay in uniform registers.
+APUS_DEV void tma_load_3d_warp(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+        " @e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n}"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+APUS_DEV void expect_tx_warp(uint64_t *bar, uint32_t bytes) {
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// A bounded wait.
+APUS_DEV bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *ab) {
+    return mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
+}
+
+// An item: ROWS query rows from r0 on of a sequence, for one head.  n < 0: no more.
+struct PaItem { int q0, n, k0, m, r0, head, first; };     // first: of the whole call
+
+// Key tiles of each query tile, the first of them with keys that some row must
+// not see, and the first that is looked after.
+template <int NQ> struct PaTiles { int nt[NQ], first_mask[NQ], mask_from, ntmax; };
+template <int NQ> APUS_DEV PaTiles<NQ> pa_tiles(const PaItem &it) {
+    PaTiles<NQ> t;
+    t.mask_from = 0x7fffffff;
+    t.ntmax = 0;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const int ra = it.r0 + i * pa::BM, rb = min(ra + pa::BM, it.n);
+        t.nt[i] = t.first_mask[i] = 0;
+        if (ra < it.n) {
+            t.nt[i] = (max(0, min(it.m, it.m - it.n + rb)) + pa::BN - 1) / pa::BN;
+            t.first_mask[i] = max(0, min(it.m, it.m - it.n + ra + 1)) / pa::BN;
+            if (t.nt[i] > 0) t.mask_from = min(t.mask_from, t.first_mask[i]);
+        }
+        t.ntmax = max(t.ntmax, t.nt[i]);
+    }
+    return t;
+}
+
 template <int D>
 __global__ void __launch_bounds__(pa::Cfg<D>::THREADS, 1)
 k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -103,28 +159,33 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     using C = pa::Cfg<D>;
     constexpr int NQ = C::NQ, NST = C::NST, PARTS = C::PARTS;
     extern __shared__ __align__(1024) uint8_t pa_dyn[];
-    __shared__ __align__(8) uint64_t q_full[PARTS], full[NST], empty[NST], checked[NST], s_free, s_full[2], p_full[2], o_done[2];
+    __shared__ __align__(16) uint4 clc_answer;
+    __shared__ __align__(8) uint64_t q_full[PARTS], q_empty, full[NST], empty[NST], checked[NST], s_free, s_full[2],
+        p_full[2], o_done[2], item_full[2], item_empty[2], clc_full;
+    __shared__ PaItem items[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, poison, found_s[2], wsum[C::THREADS / 32];
+    __shared__ int abort_flag, poison[2];
     // first key (from the first looked after, 1023: none) with a NaN, +inf, -inf in
-    // a dim, ten bits each; at most four tiles are looked after
-    __shared__ uint32_t first_bad[D];
+    // a dim, ten bits each; at most four tiles are looked after.  Items take turns.
+    __shared__ uint32_t first_bad[2][D];
     // (a shuffle tells the compiler that it is the same for the warp, so that the
     // products' operands stay in uniform registers)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
-    // ---- this CTA's rows: blocks of ROWS rows, a sequence's last block (the one
-    // with the most keys) first
-    const int head = (int)(blockIdx.x % (unsigned)a.heads), block = (int)(blockIdx.x / (unsigned)a.heads);
-    if (tid == 0) found_s[0] = -1;
-    for (int i = tid; i < D; i += C::THREADS) first_bad[i] = 0x3fffffffu;
     if (tid == 0) {
         for (int p = 0; p < PARTS; p++) mbar_init(&q_full[p], 1);
+        mbar_init(&q_empty, 1);
         for (int s = 0; s < NST; s++) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); mbar_init(&checked[s], 1); }   // empty: products, scan
         mbar_init(&s_free, 128);
-        for (int i = 0; i < 2; i++) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_done[i], 1); }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_done[i], 1);
+            mbar_init(&item_full[i], 1);
+            mbar_init(&item_empty[i], C::THREADS / 32 - 1);
+        }
+        mbar_init(&clc_full, 1);
         abort_flag = 0;
-        poison = 0;
         fence_barrier_init();
     }
     if (warp == 2) {
@@ -132,53 +193,19 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                      ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    {
-        int before = 0;
-        for (int s0 = 0; s0 < a.nseq && before <= block; s0 += C::THREADS) {
-            const int s = s0 + tid;
-            const int w = s < a.nseq ? (prompt_seq(a, s, blockIdx.x == 0).n + C::ROWS - 1) / C::ROWS : 0;
-            int incl = w;
+    // warp 0: 32 sequences from c0 on, a lane's with its blocks of rows; `before`: blocks before them
+    PromptSeq cs{0, 0, 0, 0};
+    int c0 = 0, before = 0, cw = 0, cincl = 0;
+    auto chunk = [&]() {
+        cs = c0 + lane < a.nseq ? prompt_seq(a, c0 + lane, true) : PromptSeq{0, 0, 0, 0};
+        cw = cincl = (cs.n + C::ROWS - 1) / C::ROWS;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, incl, off);
-                if (lane >= off) incl += o;
-            }
-            if (lane == 31) wsum[warp] = incl;
-            __syncthreads();
-            int at = before + incl - w;
-            for (int k = 0; k < C::THREADS / 32; k++) {
-                if (k < warp) at += wsum[k];
-                before += wsum[k];
-            }
-            if (at <= block && block < at + w) { found_s[0] = s; found_s[1] = w - 1 - (block - at); }
-            __syncthreads();
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, cincl, off);
+            if (lane >= off) cincl += o;
         }
-    }
-    if (found_s[0] < 0) {
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        if (warp == 2)
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(512) : "memory");
-        return;
-    }
-    const PromptSeq sq = prompt_seq(a, found_s[0], false);
-    const int r0 = found_s[1] * C::ROWS;                    // first row of the block, in the sequence
-    const int khead = head / a.group;
-    // key tiles of each query tile, the first of them with keys that a row must
-    // not see, and the first that is looked after
-    int nt[2] = {0, 0}, first_mask[2] = {0, 0}, mask_from = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < NQ; i++) {
-        const int ra = r0 + i * pa::BM, rb = min(ra + pa::BM, sq.n);
-        if (ra < sq.n) {
-            nt[i] = (max(0, min(sq.m, sq.m - sq.n + rb)) + pa::BN - 1) / pa::BN;
-            first_mask[i] = max(0, min(sq.m, sq.m - sq.n + ra + 1)) / pa::BN;
-            if (nt[i] > 0) mask_from = min(mask_from, first_mask[i]);
-        }
-    }
-    const int ntmax = max(nt[0], nt[1]);
-
+    };
+    if (warp == 0) chunk();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -186,296 +213,469 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     volatile int *ab = &abort_flag;
     uint8_t *qs = pa_dyn + ((1024 - (smem_u32(pa_dyn) & 1023)) & 1023), *ring = qs + NQ * C::QTILE;
 
-    // The ring holds K 0, K 1, V 0, K 2, V 1, ..., the order in which they are
-    // used.  is_v, tile of ring entry e (each PARTS stages).
-    const int entries = 2 * ntmax;
-    // The P of query tile i and key tile j: one place a query tile, or (NQ 1) two
-    // that take turns; its barriers p_full and o_done and how often they were used.
-    auto p_at = [](int i, int j) { return NQ == 2 ? i : (j & 1); };
-    auto p_use = [](int j) { return NQ == 2 ? j : (j >> 1); };
-    auto entry = [&](int e, bool &is_v, int &tile) {
+    // The next item (whole warp; not warp 0): false behind the last.  A softmax warp
+    // gives its place back (done_with) when it is through with it, so whoever has
+    // item k + 2 knows that the rows of item k are written.
+    auto done_with = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[k & 1]);
+    };
+    auto next_item = [&](int k, PaItem &it) -> bool {
+        const bool got = mbar_try_wait(&item_full[k & 1], (k >> 1) & 1) ||
+                         pa_wait(&item_full[k & 1], (k >> 1) & 1, ab);
+        if (!__all_sync(0xffffffffu, got)) return false;
+        it = items[k & 1];
+        if (warp < 4) done_with(k);
+        return __all_sync(0xffffffffu, it.n >= 0);      // (a vote: the same for the warp, as above)
+    };
+    // The ring holds an item's K 0, K 1, V 0, K 2, V 1, ..., the order in which
+    // they are used, each PARTS stages; is_v, tile of its entry e.
+    auto entry = [](int e, int ntmax, bool &is_v, int &tile) {
         if (e == 0) { is_v = false; tile = 0; }
-        else if (e == entries - 1) { is_v = true; tile = ntmax - 1; }
+        else if (e == 2 * ntmax - 1) { is_v = true; tile = ntmax - 1; }
         else { is_v = !(e & 1); tile = is_v ? (e >> 1) - 1 : (e + 1) >> 1; }
     };
-    if (warp == 0) {
-        if (lane == 0 && ntmax > 0) {   // ---- copies
-            int g = 0;
-            bool ok = true;
+    // The P of query tile i and the CTA's use u of it: one place a query tile, or
+    // (NQ 1) two that take turns; how often that place was used before.
+    auto p_at = [](int i, unsigned u) { return NQ == 2 ? i : (int)(u & 1); };
+    auto p_use = [](unsigned u) { return NQ == 2 ? u : u >> 1; };
+
+    if (warp < 4) {
+    // Three warpgroups share 384 x 168 registers: the softmax keeps 128 scores a
+    // thread, so the first gives 80 of its up (88 x 128 + 208 x 256 = 168 x 384).
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0) {                    // ---- items and copies
+        // Blocks of ROWS rows in the order of the sequences, a sequence's last block
+        // (the one with the most keys) first; the heads of a block follow one another.
+        unsigned idx = blockIdx.x, g = 0, asked = 0;
+        int k = 0, loaded = 0;
+        bool ok = true;
+        auto ask = [&]() {              // for the next item: that of a CTA not yet begun, which then never begins
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive_expect_tx(&clc_full, 16);
+            asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                         ::"r"(smem_u32(&clc_answer)), "r"(smem_u32(&clc_full)) : "memory");
+        };
+        auto wait = [&](uint64_t *bar, unsigned parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) ok = __all_sync(0xffffffffu, pa_wait(bar, parity, ab));
+        };
+        auto publish = [&](const PaItem &it) {
+            if (k >= 2) ok = __all_sync(0xffffffffu, pa_wait(&item_empty[k & 1], ((k >> 1) - 1) & 1, ab));
+            if (ok && lane == 0) {
+                items[k & 1] = it;
+                mbar_arrive(&item_full[k & 1]);
+            }
+            k++;
+        };
+        while (true) {
+            const int head = (int)(idx % (unsigned)a.heads), block = (int)(idx / (unsigned)a.heads);
+            if (block < before) { c0 = before = 0; chunk(); }
+            int sum = __shfl_sync(0xffffffffu, cincl, 31);
+            while (block >= before + sum && c0 + 32 < a.nseq) {
+                before += sum;
+                c0 += 32;
+                chunk();
+                sum = __shfl_sync(0xffffffffu, cincl, 31);
+            }
+            bool pending = false;
+            if (block < before + sum) {
+                const int rel = block - before;
+                const int src = __ffs(__ballot_sync(0xffffffffu, cincl - cw <= rel && rel < cincl)) - 1;
+                PaItem it;
+                it.q0 = __shfl_sync(0xffffffffu, cs.q0, src);
+                it.n = __shfl_sync(0xffffffffu, cs.n, src);
+                it.k0 = __shfl_sync(0xffffffffu, cs.k0, src);
+                it.m = __shfl_sync(0xffffffffu, cs.m, src);
+                it.r0 = (__shfl_sync(0xffffffffu, cincl, src) - 1 - rel) * C::ROWS;
+                it.head = head;
+                it.first = idx == 0;
+                publish(it);
+                const int ntmax = __shfl_sync(0xffffffffu, pa_tiles<NQ>(it).ntmax, 0), khead = head / a.group, entries = 2 * ntmax;
+                const int k_row = it.k0, q_row = it.q0 + it.r0;
+                auto load_q = [&](int part) {
+                    expect_tx_warp(&q_full[part], NQ * C::STAGE);
+                    for (int i = 0; i < NQ; i++)
+                        for (int p = part * (C::SPAN / 64); p < (part + 1) * (C::SPAN / 64); p++)
+                            tma_load_3d_warp(qs + i * C::QTILE + p * pa::PANEL, &qmap, p * 64, head, q_row + i * pa::BM, &q_full[part]);
+                };
+                for (int e = 0; e < entries && ok; e++) {
+                    bool is_v;
+                    int tile;
+                    entry(e, ntmax, is_v, tile);
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++, g++) {
+                        const unsigned s = g % NST;
+                        if (g >= NST) wait(&empty[s], (g / NST - 1) & 1);
+                        if (!ok) break;
+                        expect_tx_warp(&full[s], C::STAGE);
+                        uint8_t *st = ring + s * C::STAGE;
+#pragma unroll
+                        for (int p = 0; p < C::SPAN / 64; p++)
+                            tma_load_3d_warp(st + p * pa::PANEL, is_v ? &vmap : &kmap, part * C::SPAN + p * 64, khead,
+                                             k_row + tile * pa::BN, &full[s]);
+                        // part by part, so that the first product can begin; later, Q is
+                        // the last item's until that has no more products of S
+                        if (e == 0 && loaded == 0) load_q(part);
+                    }
+                    if (e == 0 && loaded > 0 && ok) {
+                        wait(&q_empty, (loaded - 1) & 1);
+                        if (!ok) break;
+                        for (int part = 0; part < PARTS; part++) load_q(part);
+                    }
+                    // early enough that the answer is there when the copies end
+                    if (ok && e == max(0, entries - 4)) { if (lane == 0) ask(); pending = true; }
+                }
+                if (ntmax > 0) loaded++;
+            }
+            if (!ok && !pending) break;
+            int more = 0;
+            unsigned nx = 0;
+            if (lane == 0) {
+                if (!pending) ask();
+                // an answer in flight is waited for whatever happens, but not for ever
+                const long long t0 = clock64();
+                while (!mbar_try_wait(&clc_full, asked & 1))
+                    if (clock64() - t0 > (1ll << 31)) {
+                        abort_flag = 1;
+                        atomicExch(&g_pa_err, (int)ATTN_ERR_WAIT);
+                        ok = false;
+                        break;
+                    }
+                if (ok)
+                    asm volatile(
+                        "{\n .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%2];\n"
+                        " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.b32 %0, 1, 0, p;\n"
+                        " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}"
+                        : "=r"(more), "+r"(nx) : "r"(smem_u32(&clc_answer)) : "memory");
+            }
+            asked++;
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            more = __shfl_sync(0xffffffffu, more, 0);
+            idx = __shfl_sync(0xffffffffu, nx, 0);
+            if (!ok || !more) break;
+        }
+        if (ok) publish(PaItem{0, -1, 0, 0, 0, 0, 0});
+    } else if (warp == 1) {             // ---- S = Q . K^T (the whole warp, one elected lane issuing)
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, unsigned parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+                ok = __all_sync(0xffffffffu, pa_wait(bar, parity, ab));
+        };
+        PaItem it;
+        unsigned use = 0, g0 = 0, loaded = 0;
+        for (int k = 0; ok && next_item(k, it); k++) {
+            const PaTiles<NQ> t = pa_tiles<NQ>(it);
+            const int n0 = __shfl_sync(0xffffffffu, t.nt[0], 0), n1 = __shfl_sync(0xffffffffu, NQ == 2 ? t.nt[NQ - 1] : 0, 0);
+            const int n = max(n0, n1);
+            g0 = __shfl_sync(0xffffffffu, g0, 0);
+            use = __shfl_sync(0xffffffffu, use, 0);
+            loaded = __shfl_sync(0xffffffffu, loaded, 0);
+            // The uses of S: key tile j of query tile 0, then of query tile 1, while they
+            // have tiles left.  S is free again as soon as a softmax has it in registers,
+            // so the softmax that ends finds its next S there.
+            for (int j = 0; j < n && ok; j++)
+#pragma unroll
+                for (int i = 0; i < NQ; i++) {
+                    if (!ok || j >= (i == 0 ? n0 : n1)) continue;
+                    const bool first = i == 0 || j >= n0, last = i == NQ - 1 || j >= n1;   // to use this K tile
+                    if (use > 0) wait(&s_free, (use - 1) & 1);
+                    tc_fence_after();
+                    use++;
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++) {
+                        const unsigned gg = g0 + (unsigned)((j == 0 ? 0 : 2 * j - 1) * PARTS + part);
+                        if (j == 0 && first) wait(&q_full[part], loaded & 1);
+                        if (first) wait(&full[gg % NST], (gg / NST) & 1);
+                        if (!ok) break;
+                        const uint32_t kb = smem_u32(ring) + (gg % NST) * C::STAGE;
+                        const uint32_t qb = smem_u32(qs) + i * C::QTILE + part * (C::SPAN / 64) * pa::PANEL;
+#pragma unroll
+                        for (int kk = 0; kk < C::SPAN / 16; kk++) {
+                            const uint32_t off = (kk >> 2) * pa::PANEL + (kk & 3) * 32;
+                            tc_mma_warp(tmem, umma_desc_sw128(qb + off), umma_desc_sw128(kb + off), C::IDESC_S, (part | kk) != 0);
+                        }
+                        if (last) tc_commit_warp(&empty[gg % NST]);
+                    }
+                    if (ok) tc_commit_warp(&s_full[i]);
+                }
+            if (ok && n > 0) {
+                tc_commit_warp(&q_empty);
+                loaded++;
+            }
+            g0 += (unsigned)(2 * n * PARTS);
+        }
+    } else if (warp == 3) {             // ---- O += P . V
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, unsigned parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+                ok = __all_sync(0xffffffffu, pa_wait(bar, parity, ab));
+        };
+        PaItem it;
+        unsigned g0 = 0, used[2] = {0, 0};
+        for (int k = 0; ok && next_item(k, it); k++) {
+            const PaTiles<NQ> t = pa_tiles<NQ>(it);
+            const int n0 = __shfl_sync(0xffffffffu, t.nt[0], 0), n1 = __shfl_sync(0xffffffffu, NQ == 2 ? t.nt[NQ - 1] : 0, 0);
+            const int mf = __shfl_sync(0xffffffffu, t.mask_from, 0), n = max(n0, n1);
+            g0 = __shfl_sync(0xffffffffu, g0, 0);
+            used[0] = __shfl_sync(0xffffffffu, used[0], 0); used[1] = __shfl_sync(0xffffffffu, used[1], 0);
+            for (int j = 0; j < n && ok; j++)
+#pragma unroll
+                for (int i = 0; i < NQ; i++) {
+                    if (!ok || j >= (i == 0 ? n0 : n1)) continue;
+                    const bool first = i == 0 || j >= n0, last = i == NQ - 1 || j >= n1;   // to use this V tile
+                    const unsigned u = used[i]++;
+                    wait(&p_full[p_at(i, u)], p_use(u) & 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++) {
+                        const unsigned gg = g0 + (unsigned)((j == n - 1 ? 2 * n - 1 : 2 * j + 2) * PARTS + part);
+                        if (first) wait(&full[gg % NST], (gg / NST) & 1);
+                        if (first && j >= mf) wait(&checked[gg % NST], (gg / NST) & 1);
+                        if (!ok) break;
+                        const uint32_t vb = smem_u32(ring) + (gg % NST) * C::STAGE;
+#pragma unroll
+                        for (int kk = 0; kk < pa::BN / 16; kk++)
+                            tc_mma_ts_warp(tmem + C::O_COL + i * D + part * C::SPAN, tmem + C::P_COL + p_at(i, u) * 64 + kk * 8,
+                                           umma_desc_mn_sw128(vb + kk * 2048, pa::PANEL), C::IDESC_O,
+                                           kk ? 1u : (uint32_t)(j > 0));
+                        if (last) tc_commit_warp(&empty[gg % NST]);
+                    }
+                    if (ok) tc_commit_warp(&o_done[p_at(i, u)]);
+                }
+            g0 += (unsigned)(2 * n * PARTS);
+        }
+    } else {                            // ---- V tiles with hidden keys
+        unsigned g = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, unsigned parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) ok = __all_sync(0xffffffffu, pa_wait(bar, parity, ab));
+        };
+        PaItem it;
+        for (int k = 0; ok && next_item(k, it); k++) {
+            const PaTiles<NQ> t = pa_tiles<NQ>(it);
+            // sequences out of bounds behind the last one with rows are reported too
+            if (it.first)
+#pragma unroll 4
+                for (int s = 32 + lane; s < a.nseq; s += 32) prompt_seq(a, s, true);
+            uint32_t *const bad_key = first_bad[k & 1];
+            for (int i = lane; i < D; i += 32) bad_key[i] = 0x3fffffffu;
+            if (lane == 0) poison[k & 1] = 0;
+            __syncwarp();
+            const int ntmax = __shfl_sync(0xffffffffu, t.ntmax, 0), entries = 2 * ntmax;
+            const int mask_from = __shfl_sync(0xffffffffu, t.mask_from, 0);
+            g = __shfl_sync(0xffffffffu, g, 0);
             for (int e = 0; e < entries && ok; e++) {
                 bool is_v;
                 int tile;
-                entry(e, is_v, tile);
-                for (int part = 0; part < PARTS && ok; part++, g++) {
-                    const int s = g % NST;
-                    if (e == 0) {       // this part of Q, then of the first K: the first product can begin
-                        mbar_arrive_expect_tx(&q_full[part], NQ * C::STAGE);
-                        for (int i = 0; i < NQ; i++)
-                            for (int p = part * (C::SPAN / 64); p < (part + 1) * (C::SPAN / 64); p++)
-                                tma_load_3d(qs + i * C::QTILE + p * pa::PANEL, &qmap, p * 64, head,
-                                            sq.q0 + r0 + i * pa::BM, &q_full[part]);
-                    }
-                    if (g >= NST && !(ok = mbar_wait(&empty[s], ((g / NST) - 1) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT))) break;
-                    mbar_arrive_expect_tx(&full[s], C::STAGE);
-                    for (int p = 0; p < C::SPAN / 64; p++)
-                        tma_load_3d(ring + s * C::STAGE + p * pa::PANEL, is_v ? &vmap : &kmap, part * C::SPAN + p * 64, khead,
-                                    sq.k0 + tile * pa::BN, &full[s]);
-                }
-            }
-        }
-    } else if (warp == 1) {             // ---- S = Q . K^T (the whole warp, one elected lane issuing)
-        const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
-        bool ok = true;
-        auto wait = [&](uint64_t *bar, int parity) {
-            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
-        };
-        // The uses of S: key tile j of query tile 0, then of query tile 1, while they
-        // have tiles left.  S is free again as soon as a softmax has it in registers,
-        // so the softmax that ends finds its next S there.
-        int use = 0;
-        for (int j = 0; j < max(n0, n1) && ok; j++)
-#pragma unroll
-            for (int i = 0; i < NQ; i++) {
-                if (!ok || j >= (i == 0 ? n0 : n1)) continue;
-                const bool first = i == 0 || j >= n0, last = i == NQ - 1 || j >= n1;   // to use this K tile
-                if (use > 0) wait(&s_free, (use - 1) & 1);
-                tc_fence_after();
-                use++;
-#pragma unroll
-                for (int part = 0; part < PARTS; part++) {
-                    const int gg = (j == 0 ? 0 : 2 * j - 1) * PARTS + part;
-                    if (use == 1) wait(&q_full[part], 0);
-                    if (first) wait(&full[gg % NST], (gg / NST) & 1);
+                entry(e, ntmax, is_v, tile);
+                for (int part = 0; part < PARTS; part++, g++) {
+                    const unsigned s = g % NST;
+                    wait(&full[s], (g / NST) & 1);
                     if (!ok) break;
-                    const uint32_t kb = smem_u32(ring) + (gg % NST) * C::STAGE;
-                    const uint32_t qb = smem_u32(qs) + i * C::QTILE + part * (C::SPAN / 64) * pa::PANEL;
+                    if (is_v && tile >= mask_from) {
+                        uint8_t *st = ring + s * C::STAGE;
+                        const int key0 = tile * pa::BN;
+                        const int behind = it.m - key0;                 // rows from here on belong to no key
+                        // eight 16-byte pieces at a time: an exponent of all ones carries
+                        // into the sign bit
+                        for (int i = lane * 16; i < C::STAGE; i += 8 * 32 * 16) {
+                            uint4 w[8];
 #pragma unroll
-                    for (int k = 0; k < C::SPAN / 16; k++) {
-                        const uint32_t off = (k >> 2) * pa::PANEL + (k & 3) * 32;
-                        tc_mma_warp(tmem, umma_desc_sw128(qb + off), umma_desc_sw128(kb + off), C::IDESC_S, (part | k) != 0);
-                    }
-                    if (last) tc_commit_warp(&empty[gg % NST]);
-                }
-                if (ok) tc_commit_warp(&s_full[i]);
-            }
-    } else if (warp == 3) {             // ---- O += P . V
-        const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0);
-        const int mf = __shfl_sync(0xffffffffu, mask_from, 0), n = max(n0, n1);
-        bool ok = true;
-        auto wait = [&](uint64_t *bar, int parity) {
-            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
-        };
-        for (int j = 0; j < n && ok; j++)
+                            for (int u = 0; u < 8; u++) w[u] = lds128(st + i + u * 512);
+                            if (behind < pa::BN) {
 #pragma unroll
-            for (int i = 0; i < NQ; i++) {
-                if (!ok || j >= (i == 0 ? n0 : n1)) continue;
-                const bool first = i == 0 || j >= n0, last = i == NQ - 1 || j >= n1;   // to use this V tile
-                wait(&p_full[p_at(i, j)], p_use(j) & 1);
-                tc_fence_after();
+                                for (int u = 0; u < 8; u++)
+                                    if ((((i + u * 512) / 128) & 127) >= behind) {
+                                        w[u] = make_uint4(0, 0, 0, 0);
+                                        *(uint4 *)(st + i + u * 512) = w[u];
+                                    }
+                            }
+                            uint32_t bad = 0;
 #pragma unroll
-                for (int part = 0; part < PARTS; part++) {
-                    const int gg = (j == n - 1 ? 2 * n - 1 : 2 * j + 2) * PARTS + part;
-                    if (first) wait(&full[gg % NST], (gg / NST) & 1);
-                    if (first && j >= mf) wait(&checked[gg % NST], (gg / NST) & 1);
-                    if (!ok) break;
-                    const uint32_t vb = smem_u32(ring) + (gg % NST) * C::STAGE;
-#pragma unroll
-                    for (int k = 0; k < pa::BN / 16; k++)
-                        tc_mma_ts_warp(tmem + C::O_COL + i * D + part * C::SPAN, tmem + C::P_COL + p_at(i, j) * 64 + k * 8,
-                                       umma_desc_mn_sw128(vb + k * 2048, pa::PANEL), C::IDESC_O, k ? 1u : (uint32_t)(j > 0));
-                    if (last) tc_commit_warp(&empty[gg % NST]);
-                }
-                if (ok) tc_commit_warp(&o_done[p_at(i, j)]);
-            }
-    } else if (warp == 2) {             // ---- V tiles with hidden keys
-        int g = 0;
-        bool ok = true;
-        for (int e = 0; e < entries && ok; e++) {
-            bool is_v;
-            int tile;
-            entry(e, is_v, tile);
-            for (int part = 0; part < PARTS; part++, g++) {
-                const int s = g % NST;
-                const bool got = mbar_wait(&full[s], (g / NST) & 1, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
-                ok = __all_sync(0xffffffffu, got);
-                if (!ok) break;
-                if (is_v && tile >= mask_from) {
-                    uint8_t *st = ring + s * C::STAGE;
-                    const int behind = sq.m - tile * pa::BN;        // rows from here on belong to no key
-                    // eight 16-byte pieces at a time: an exponent of all ones carries
-                    // into the sign bit
-                    for (int i = lane * 16; i < C::STAGE; i += 8 * 32 * 16) {
-                        uint4 w[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) w[k] = lds128(st + i + k * 512);
-                        if (behind < pa::BN) {
-#pragma unroll
-                            for (int k = 0; k < 8; k++)
-                                if ((((i + k * 512) / 128) & 127) >= behind) {
-                                    w[k] = make_uint4(0, 0, 0, 0);
-                                    *(uint4 *)(st + i + k * 512) = w[k];
-                                }
-                        }
-                        uint32_t bad = 0;
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            bad |= ((w[k].x & 0x7f807f80u) + 0x00800080u) | ((w[k].y & 0x7f807f80u) + 0x00800080u) |
-                                   ((w[k].z & 0x7f807f80u) + 0x00800080u) | ((w[k].w & 0x7f807f80u) + 0x00800080u);
-                        if (!(bad & 0x80008000u)) continue;
+                            for (int u = 0; u < 8; u++)
+                                bad |= ((w[u].x & 0x7f807f80u) + 0x00800080u) | ((w[u].y & 0x7f807f80u) + 0x00800080u) |
+                                       ((w[u].z & 0x7f807f80u) + 0x00800080u) | ((w[u].w & 0x7f807f80u) + 0x00800080u);
+                            if (!(bad & 0x80008000u)) continue;
 #pragma unroll 1
-                        for (int k = 0; k < 8; k++) {
-                            const int at = i + k * 512, r = (at / 128) & 127;
-                            // the piece's place in its row is swizzled by the row
-                            const int d0 = part * C::SPAN + (at / pa::PANEL) * 64 + (((at >> 4) & 7) ^ (r & 7)) * 8;
-                            uint16_t *h = (uint16_t *)(st + at);
                             for (int u = 0; u < 8; u++) {
-                                const uint16_t x = h[u];
-                                if ((x & 0x7f80) != 0x7f80) continue;
-                                h[u] = 0;
-                                const int sh = ((x & 0x7f) ? 0 : (x >> 15) ? 2 : 1) * 10;
-                                const uint32_t key = (uint32_t)((tile - mask_from) * pa::BN + r);
-                                uint32_t old = first_bad[d0 + u], was;
-                                while (key < ((old >> sh) & 1023u)) {
-                                    was = old;
-                                    old = atomicCAS(&first_bad[d0 + u], was, (was & ~(1023u << sh)) | (key << sh));
-                                    if (old == was) break;
+                                const int at = i + u * 512, r = (at / 128) & 127;
+                                // the piece's place in its row is swizzled by the row
+                                const int d0 = part * C::SPAN + (at / pa::PANEL) * 64 + (((at >> 4) & 7) ^ (r & 7)) * 8;
+                                uint16_t *h = (uint16_t *)(st + at);
+                                for (int x8 = 0; x8 < 8; x8++) {
+                                    const uint16_t x = h[x8];
+                                    if ((x & 0x7f80) != 0x7f80) continue;
+                                    h[x8] = 0;
+                                    const int sh = ((x & 0x7f) ? 0 : (x >> 15) ? 2 : 1) * 10;
+                                    const uint32_t key = (uint32_t)(key0 - mask_from * pa::BN + r);
+                                    uint32_t old = bad_key[d0 + x8], was;
+                                    while (key < ((old >> sh) & 1023u)) {
+                                        was = old;
+                                        old = atomicCAS(&bad_key[d0 + x8], was, (was & ~(1023u << sh)) | (key << sh));
+                                        if (old == was) break;
+                                    }
+                                    poison[k & 1] = 1;
                                 }
-                                poison = 1;
                             }
                         }
+                        static_assert(C::STAGE % (8 * 32 * 16) == 0, "whole batches of pieces");
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
-                    static_assert(C::STAGE % (8 * 32 * 16) == 0, "whole batches of pieces");
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&checked[s]);
-                    mbar_arrive(&empty[s]);
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&checked[s]);
+                        mbar_arrive(&empty[s]);
+                    }
                 }
             }
         }
+    }
     } else {                            // ---- softmax, one row a thread
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int i = (warp - 4) >> 2;                      // query tile
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const int rt = (warp & 3) * 32 + lane, row = r0 + i * pa::BM + rt;      // row in the sequence
-        const int nti = nt[i];
-        const int seen = max(0, min(sq.m, sq.m - sq.n + min(row, sq.n - 1) + 1));   // keys that it sees
         const uint32_t o_col = tmem + lanes + C::O_COL + i * D;
-        float m = -INFINITY, l = 0.f;
         const float raise = pa::RAISE / a.zscale;
         bool ok = true;
-        auto wait = [&](uint64_t *bar, int parity) {
+        auto wait = [&](uint64_t *bar, unsigned parity) {
             if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT));
+                ok = __all_sync(0xffffffffu, pa_wait(bar, parity, ab));
             tc_fence_after();
         };
-        for (int j = 0; j < nti; j++) {
-            wait(&s_full[i], j & 1);
-            if (!ok) break;
-            float v[128];
-            tc_ld128(tmem + lanes, v);
-            tc_fence_before();
-            mbar_arrive(&s_free);
-            if (j >= first_mask[i]) {
-                const int lim = seen - j * pa::BN;
-#pragma unroll
-                for (int c = 0; c < 128; c++) v[c] = c < lim ? v[c] : -INFINITY;
+        unsigned used = 0;              // key tiles of the items before
+        for (int k = 0; ok; k++) {
+            int nti, first_mask, seen;
+            {
+                PaItem it;
+                if (!next_item(k, it)) break;
+                const PaTiles<NQ> t = pa_tiles<NQ>(it);
+                nti = __shfl_sync(0xffffffffu, i == 0 ? t.nt[0] : t.nt[NQ - 1], 0);
+                first_mask = __shfl_sync(0xffffffffu, i == 0 ? t.first_mask[0] : t.first_mask[NQ - 1], 0);
+                used = __shfl_sync(0xffffffffu, used, 0);
+                const int row = it.r0 + i * pa::BM + (warp & 3) * 32 + lane;    // row in the sequence
+                seen = max(0, min(it.m, it.m - it.n + min(row, it.n - 1) + 1));       // keys that it sees
             }
-            float mx[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-            for (int c = 4; c < 128; c += 4)
-#pragma unroll
-                for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], v[c + u]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            const bool up = top > m + raise;
-            if (__any_sync(0xffffffffu, up)) {
-                const float down = !up ? 1.0f : m == -INFINITY ? 0.f : pa_ex2((m - top) * a.zscale);
-                if (up) m = top;
-                l *= down;
-                if (j > 0) {                 // O is the product's of j - 1 until that is done
-                    wait(&o_done[p_at(i, j - 1)], p_use(j - 1) & 1);
-                    if (!ok) break;
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tc_ld32(o_col + c, o);
-#pragma unroll
-                        for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * down);
-                        tc_st32(o_col + c, o);
-                    }
-                }
-            }
-            const float mz = m == -INFINITY ? 0.f : m * a.zscale;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t pk[2][32];
-#pragma unroll
-            for (int c = 0; c < 128; c += 2) {
-                const float p0 = pa_ex2(fmaf(v[c], a.zscale, -mz)), p1 = pa_ex2(fmaf(v[c + 1], a.zscale, -mz));
-                sum[c & 2] += p0;
-                sum[(c & 2) + 1] += p1;
-                pk[c / 64][(c % 64) / 2] = pa_pack(p0, p1);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            // P's place is read by the product of j - 1 (NQ 1: j - 2) until that is done
-            if (j >= (NQ == 2 ? 1 : 2)) {
-                wait(&o_done[p_at(i, j)], (p_use(j) - 1) & 1);
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < nti; j++) {
+                const unsigned u = used + (unsigned)j;
+                wait(&s_full[i], u & 1);
                 if (!ok) break;
-            }
-            const uint32_t p_col = tmem + lanes + C::P_COL + p_at(i, j) * 64;
-            tc_st32(p_col, pk[0]);
-            tc_st32(p_col + 32, pk[1]);
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[p_at(i, j)]);
-        }
-        if (NQ == 1 && ok && nti > 1) wait(&o_done[p_at(i, nti - 2)], p_use(nti - 2) & 1);
-        if (ok && nti > 0) wait(&o_done[p_at(i, nti - 1)], p_use(nti - 1) & 1);
-        // a query tile that sees no key: its rows of Q may still be on their way
-        if (nti == 0 && ntmax > 0)
-            for (int p = 0; p < PARTS; p++) wait(&q_full[p], 0);
-        if (ok) {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
-            // through this warp's rows of the Q tile, which nothing reads any more, so
-            // that rows are stored whole: 16-byte pieces, swizzled by the row
-            uint8_t *own = qs + i * C::QTILE + (warp & 3) * 32 * (D * 2);
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                if (nti > 0) tc_ld32(o_col + c, o);
-                if (*(volatile int *)&poison) {
+                float v[128];
+                tc_ld128(tmem + lanes, v);
+                tc_fence_before();
+                mbar_arrive(&s_free);
+                if (j >= first_mask) {
+                    const int lim = seen - j * pa::BN;
 #pragma unroll
-                    for (int u = 0; u < 32; u++) {
-                        float x = __uint_as_float(o[u]);
-                        const uint32_t f = first_bad[c + u];
-                        const int rel = seen - mask_from * pa::BN;       // looked-after keys that the row sees
-                        if (rel > (int)(f & 1023u)) x = __int_as_float(0x7fc00000);
-                        if (rel > (int)((f >> 10) & 1023u)) x += INFINITY;
-                        if (rel > (int)(f >> 20)) x -= INFINITY;
-                        o[u] = __float_as_uint(x);
+                    for (int c = 0; c < 128; c++) v[c] = c < lim ? v[c] : -INFINITY;
+                }
+                float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int c = 4; c < 128; c += 4)
+#pragma unroll
+                    for (int h = 0; h < 4; h++) mx[h] = fmaxf(mx[h], v[c + h]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool up = top > m + raise;
+                if (__any_sync(0xffffffffu, up)) {
+                    const float down = !up ? 1.0f : m == -INFINITY ? 0.f : pa_ex2((m - top) * a.zscale);
+                    if (up) m = top;
+                    l *= down;
+                    if (j > 0) {                 // O is the product's of j - 1 until that is done
+                        wait(&o_done[p_at(i, u - 1)], p_use(u - 1) & 1);
+                        if (!ok) break;
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tc_ld32(o_col + c, o);
+#pragma unroll
+                            for (int h = 0; h < 32; h++) o[h] = __float_as_uint(__uint_as_float(o[h]) * down);
+                            tc_st32(o_col + c, o);
+                        }
                     }
                 }
+                const float mz = m == -INFINITY ? 0.f : m * a.zscale;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t pk[2][32];
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-                        w[u] = nti > 0 ? pa_pack(__uint_as_float(o[8 * h + 2 * u]) * inv,
-                                                 __uint_as_float(o[8 * h + 2 * u + 1]) * inv) : 0u;
-                    *(uint4 *)(own + lane * (D * 2) + (((c / 8 + h) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int c = 0; c < 128; c += 2) {
+                    const float p0 = pa_ex2(fmaf(v[c], a.zscale, -mz)), p1 = pa_ex2(fmaf(v[c + 1], a.zscale, -mz));
+                    sum[c & 2] += p0;
+                    sum[(c & 2) + 1] += p1;
+                    pk[c / 64][(c % 64) / 2] = pa_pack(p0, p1);
                 }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                // P's place is read by the product of its last use until that is done
+                if (p_use(u) > 0) {
+                    wait(&o_done[p_at(i, u)], (p_use(u) - 1) & 1);
+                    if (!ok) break;
+                }
+                const uint32_t p_col = tmem + lanes + C::P_COL + p_at(i, u) * 64;
+                tc_st32(p_col, pk[0]);
+                tc_st32(p_col + 32, pk[1]);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[p_at(i, u)]);
             }
-            __syncwarp();
-            constexpr int PIECES = D / 8, RPS = 32 / PIECES > 0 ? 32 / PIECES : 1;     // pieces of a row, rows of a store
-            const int left = sq.n - (row - lane);                                      // rows of this warp that exist
-#pragma unroll 4
-            for (int r = 0; r < 32; r += RPS) {
-                const int rr = r + (RPS > 1 ? lane / PIECES : 0), p = RPS > 1 ? lane % PIECES : lane;
-                if (rr < left)
-                    *(uint4 *)(a.out.p + (long)(sq.q0 + row - lane + rr) * a.out.rs + (long)head * a.out.hs + p * 8) =
-                        lds128(own + rr * (D * 2) + ((p ^ (rr & 7)) << 4));
+            used += (unsigned)nti;
+            if (NQ == 1 && ok && nti > 1) wait(&o_done[p_at(i, used - 2)], p_use(used - 2) & 1);
+            if (ok && nti > 0) wait(&o_done[p_at(i, used - 1)], p_use(used - 1) & 1);
+            if (!ok) break;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            // (the addresses below are the same for every item: kept out of the registers
+            // of the loop above, which has none left)
+            int ln = lane;
+            asm volatile("" : "+r"(ln));
+            uint8_t *const own = ring + NST * C::STAGE + (warp - 4) * C::OUT;
+            const PaItem it = items[k & 1];
+            int mask_from;
+            bool bad;
+            {
+                const PaTiles<NQ> t = pa_tiles<NQ>(it);
+                mask_from = t.mask_from;
+                bad = mask_from < t.ntmax && *(volatile int *)&poison[k & 1];
             }
+            const int row0 = it.r0 + i * pa::BM + (warp & 3) * 32, left = it.n - row0;      // this warp's first row, rows that exist
+            uint16_t *const op = a.out.p + (long)(it.q0 + row0) * a.out.rs + (long)it.head * a.out.hs;
+            // through shared memory, so that a store covers 128 bytes of four rows:
+            // 16-byte pieces, swizzled by the row
+#pragma unroll 1
+            for (int c = 0; c < D; c += 64) {
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    uint32_t o[32];
+                    if (nti > 0) tc_ld32(o_col + c + half * 32, o);
+                    else
+#pragma unroll
+                        for (int h = 0; h < 32; h++) o[h] = 0;
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            w[x] = pa_pack(__uint_as_float(o[8 * h + 2 * x]) * inv, __uint_as_float(o[8 * h + 2 * x + 1]) * inv);
+                        *(uint4 *)(own + ln * 128 + (((half * 4 + h) ^ (ln & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                if (bad)
+#pragma unroll 1
+                    for (int d = 0; d < 64; d++) {
+                        const uint32_t f = first_bad[k & 1][c + d];
+                        const int rel = seen - mask_from * pa::BN;       // looked-after keys that the row sees
+                        uint16_t *o = (uint16_t *)(own + ln * 128 + (((d >> 3) ^ (ln & 7)) << 4)) + (d & 7);
+                        const bool pos = rel > (int)((f >> 10) & 1023u), neg = rel > (int)(f >> 20);
+                        if (rel > (int)(f & 1023u) || (pos && (neg || *o == 0xff80)) || (neg && *o == 0x7f80)) *o = 0x7fff;
+                        else if ((pos || neg) && (*o & 0x7fff) <= 0x7f80) *o = pos ? 0x7f80 : 0xff80;
+                    }
+                __syncwarp();
+#pragma unroll
+                for (int r = 0; r < 32; r += 4) {
+                    const int rr = r + (ln >> 3), piece = ln & 7;
+                    if (rr < left) *(uint4 *)(op + (long)rr * a.out.rs + c + piece * 8) = lds128(own + rr * 128 + ((piece ^ (rr & 7)) << 4));
+                }
+                __syncwarp();
+            }
+            tc_fence_before();          // before the next item's first product writes O (after this thread's next p_full)
+            done_with(k);
         }
     }
     tc_fence_before();

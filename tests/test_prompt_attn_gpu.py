@@ -126,6 +126,34 @@ def test_unseen_keys_have_no_influence(gcuda, dim):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dim,heads,group", [(64, 4, 8), (128, 4, 8), (256, 16, 2)])
+def test_many_items(gcuda, dim, heads, group):
+    """Far more blocks of rows than SMs, so that a CTA takes one after the other: over a hundred sequences of 0 to 300
+    rows over 0 to 500 keys, and the same with NaN and infinities in every third sequence's last value, which its last
+    row alone sees."""
+    g = torch.Generator().manual_seed(dim + 1)
+    rows = [int(x) for x in torch.randint(0, 301, (110,), generator=g)]
+    keys = [n + int(x) for n, x in zip(rows, torch.randint(-20, 200, (110,), generator=g))]
+    keys = [max(m, 0) for m in keys]
+    rows[40:44], keys[40:44] = [0, 0, 5, 256], [0, 9, 0, 256]
+    q = bf16(g, sum(rows) + 3, heads * group, dim).cuda()
+    k, v = (bf16(g, sum(keys) + 3, heads, dim).cuda() for _ in range(2))
+    out = run(gcuda, q, k, v, rows, keys, dim ** -0.5)
+    check(q, k, v, out, rows, keys, dim ** -0.5)
+    assert (out[sum(rows):] == 7).all()
+    v2, want = v.clone(), out.clone()
+    q0, k0 = starts(rows).tolist(), starts(keys).tolist()
+    for i in range(0, 110, 3):
+        if rows[i] and keys[i]:
+            c = i // 3 % 3
+            v2[k0[i + 1] - 1, i % heads, 7 * c] = (float("nan"), float("inf"), float("-inf"))[c]
+            want[q0[i + 1] - 1, i % heads * group:(i % heads + 1) * group, 7 * c] = (float("nan"), float("inf"), float("-inf"))[c]
+    for _ in range(2):
+        got = run(gcuda, q, k, v2, rows, keys, dim ** -0.5)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
 def test_ranges_out_of_bounds(gcuda):
     g = torch.Generator().manual_seed(10)
     q, k, v = (bf16(g, 100, 2, 64).cuda() for _ in range(3))
