@@ -374,6 +374,8 @@ def kv4_attn(cache, batch, q, out, scale, workspace=None, sel=None, pool=0, stre
     if sel is not None and (sel.dtype != torch.uint8 or sel.dim() != 2 or sel.shape[0] < q.shape[0] or
                             not sel.is_contiguous()):
         raise GcudaError(f"kv4_attn: sel is contiguous uint8 [rows][pools], not {sel.dtype} {list(sel.shape)}")
+    if workspace is not None and not workspace.is_contiguous():
+        raise GcudaError("kv4_attn: workspace is not contiguous")
     check(apus_gcuda_kv4_attn_dev(cache.ref, batch.ref, head_rows(q, "q"), head_rows(out, "out"), scale,
                                   None if sel is None else sel.data_ptr() or cache.pages.data_ptr(),
                                   0 if sel is None else sel.shape[1], pool,

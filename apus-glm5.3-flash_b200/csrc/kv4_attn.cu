@@ -30,7 +30,7 @@
 //     the mantissa of 1024 and the offset is subtracted: exact integers.
 //   * Scales are unpacked once a unit, not once a lane that needs them: fp32 for
 //     the keys; for the values f16 below 2, with a power of two a position that
-//     goes into the weight's exponent.  Two f16 roundings (2^-12) a weight.
+//     goes into the weight's exponent.  Two f16 roundings (2^-11 each) a weight.
 // (E4M3 mma.sync looks four times as fast but is carried out as conversions and
 // f16 products: 50 conversions for 16 positions of dim 128, and no faster.)
 //
@@ -44,8 +44,18 @@
 // Units come by cp.async, nine 16-byte pieces a lane: bulk copies of one or four
 // pieces a unit cost their issuing warp about 250 cycles each, as much as two
 // fragments' work.  Under a selection the positions that any of the columns keeps
-// are listed and gathered row by row, so what no column keeps is neither read
-// nor computed.
+// are listed, with a bit for each row that keeps them, and gathered row by row, so
+// what no column keeps is neither read nor computed.
+//
+// Measured (us a call; bytes that it has to read, of 6.55 TB/s): one sequence of
+// 131072 positions, 64 heads over 8 of 128: 48 (48%); 48 sequences of up to 8192,
+// 32 over 8: 69 (55%); 4 rows over 4363 positions of 64 heads of 256: 33 (38%);
+// 4 rows of 512 pools of 4 out of 32771: 46.  What bounds it is issue: 330
+// instructions for 16 positions of dim 128 (70 of them LOP3 and 20 shifts at half
+// rate: 48% of that pipe, 59% of all issue slots), and about 8 thousand cycles a
+// launch before and after the stream.  A fourth CTA an SM (128 registers, the
+// query in shared memory) took 8% longer.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_dev.h"
@@ -412,8 +422,8 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         }
         // ---- running maximum of z + E, so of what a position adds to the output:
         // its weight times 2^E, and times a scale below 2, then fits f16 with the
-        // largest at 2^5 to 2^13 whatever the scales' range (what is below 2^-37 of
-        // the largest adds nothing).  It is raised only when a score passes it by
+        // largest at 2^5 to 2^13 whatever the scales' range (what is below 2^-30 of
+        // the largest may add nothing).  It is raised only when a score passes it by
         // more than 2^13.
         uint32_t hide = 0;             // bit nt * 4 + i (MASKED)
         bool over = false;
@@ -661,7 +671,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             // in which a lane meets the key codes (dim 8 q4 + i of a group is code i
             // of its word)
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+            for (int nt = 0; nt < NT; nt++) {
                 uint32_t top = 0;
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
@@ -701,17 +711,17 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                     qs += __shfl_xor_sync(0xffffffffu, qs, 1);
                     qs += __shfl_xor_sync(0xffffffffu, qs, 2);
                     qs *= -8.0f / 16777216.0f;                               // the codes' offset
-                cinit[nt][j][0] = __shfl_sync(0xffffffffu, qs, 8 * q4);
-                cinit[nt][j][1] = __shfl_sync(0xffffffffu, qs, 8 * q4 + 4);
+                    cinit[nt][j][0] = __shfl_sync(0xffffffffu, qs, 8 * q4);
+                    cinit[nt][j][1] = __shfl_sync(0xffffffffu, qs, 8 * q4 + 4);
                 }
                 // what follows goes by the columns whose scores this lane holds
-            fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * q4);
-            fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * q4 + 4);
+                fac[nt][0] = __shfl_sync(0xffffffffu, f, 8 * q4);
+                fac[nt][1] = __shfl_sync(0xffffffffu, f, 8 * q4 + 4);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int t = row_of(a, min(c0 + nt * 8 + 2 * q4 + u, cols - 1));
-                lim[nt][u] = SEL ? 16 + lim_row0 + t - lim0 : lim_row0 + t;
-            }
+                for (int u = 0; u < 2; u++) {
+                    const int t = row_of(a, min(c0 + nt * 8 + 2 * q4 + u, cols - 1));
+                    lim[nt][u] = SEL ? 16 + lim_row0 + t - lim0 : lim_row0 + t;
+                }
             }
             if (C::QS) __syncthreads();
         }
@@ -805,57 +815,60 @@ __global__ void __launch_bounds__(128) k_kv4_join(const Kv4AttnArgs a, int cols_
     constexpr int L = D / 4, P = 128 / L;      // lanes over the dims, parts over the pieces
     extern __shared__ float kj_dyn[];          // weights of the pieces, then [P][D] sums
     __shared__ float total_s;
-    const int seq = blockIdx.z, head = blockIdx.y, c = blockIdx.x;
+    const int seq = blockIdx.z, head = blockIdx.y;
     const Kv4Work wk = kv4_work(a, seq, cols_block);
     const Kv4Seq sq = wk.sq;
     pdl_wait();                                // the partial results and the plan
-    if (c >= sq.n * a.group) return;
-    const int cb = c / cols_block, cc = c % cols_block;
-    const long runs = a.plan[0], total = a.plan[1];
-    const long b = a.plan[2 + seq] + ((long)head * wk.ncb + cb) * wk.pages, e = b + wk.pages;
-    const long i0 = ((b + 1) * runs - 1) / total, i1 = (e * runs - 1) / total;   // runs of the first and the last page
-    if (i0 == i1) return;                      // written by its only run
-    const int n = (int)(i1 - i0) + 1;
-    const size_t stride = (size_t)cols_block * (D + 2);
-    auto piece = [&](int i) { return a.part + ((size_t)(i0 + i) * 2 + (i == 0 ? 1 : 0)) * stride; };
-    float *sums = kj_dyn + KJ_RUNS;
-    if (threadIdx.x < 32) {
-        float mx = kv4::NEG_INF;
-        for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, piece(i)[cc]);
+    for (int c = blockIdx.x; c < sq.n * a.group; c += gridDim.x) {
+        const int cb = c / cols_block, cc = c % cols_block;
+        const long runs = a.plan[0], total = a.plan[1];
+        const long b = a.plan[2 + seq] + ((long)head * wk.ncb + cb) * wk.pages, e = b + wk.pages;
+        const long i0 = ((b + 1) * runs - 1) / total, i1 = (e * runs - 1) / total;   // runs of the first and the last page
+        if (i0 == i1) continue;                    // written by its only run
+        const int n = (int)(i1 - i0) + 1;
+        const size_t stride = (size_t)cols_block * (D + 2);
+        auto piece = [&](int i) { return a.part + ((size_t)(i0 + i) * 2 + (i == 0 ? 1 : 0)) * stride; };
+        float *sums = kj_dyn + KJ_RUNS;
+        if (threadIdx.x < 32) {
+            float mx = kv4::NEG_INF;
+            for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, piece(i)[cc]);
 #pragma unroll
-        for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-        float sum = 0.f;
-        for (int i = threadIdx.x; i < n; i += 32) {
-            const float mi = piece(i)[cc], li = piece(i)[cols_block + cc];
-            const float k = mi == kv4::NEG_INF && li == 0.f ? 0.f : ex2(mi - mx);
-            kj_dyn[i] = k;
-            sum += li * k;
+            for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            float sum = 0.f;
+            for (int i = threadIdx.x; i < n; i += 32) {
+                const float mi = piece(i)[cc], li = piece(i)[cols_block + cc];
+                const float k = mi == kv4::NEG_INF && li == 0.f ? 0.f : ex2(mi - mx);
+                kj_dyn[i] = k;
+                sum += li * k;
+            }
+#pragma unroll
+            for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if (threadIdx.x == 0) total_s = sum;
         }
-#pragma unroll
-        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (threadIdx.x == 0) total_s = sum;
-    }
-    __syncthreads();
-    const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+        const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = part; i < n; i += P) {
-        const float k = kj_dyn[i];
-        const float4 y = *(const float4 *)(piece(i) + 2 * cols_block + cc * D + d);
-        if (k != 0.f) { o.x += y.x * k; o.y += y.y * k; o.z += y.z * k; o.w += y.w * k; }   // 0: it saw nothing
-    }
-    *(float4 *)(sums + part * D + d) = o;
-    __syncthreads();
-    if (part) return;
+        for (int i = part; i < n; i += P) {
+            const float k = kj_dyn[i];
+            const float4 y = *(const float4 *)(piece(i) + 2 * cols_block + cc * D + d);
+            o.x += y.x * k; o.y += y.y * k; o.z += y.z * k; o.w += y.w * k;
+        }
+        *(float4 *)(sums + part * D + d) = o;
+        __syncthreads();
+        if (part == 0) {
 #pragma unroll
-    for (int i = 1; i < P; i++) {
-        const float4 y = *(const float4 *)(sums + i * D + d);
-        o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+            for (int i = 1; i < P; i++) {
+                const float4 y = *(const float4 *)(sums + i * D + d);
+                o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+            }
+            const float inv = total_s == 0.f ? 0.f : 1.0f / total_s;
+            const int t = row_of(a, c);
+            uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs + (long)(head * a.group + c - t * a.group) * a.out.hs + d;
+            *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+        }
+        __syncthreads();                           // the next column's weights and sums
     }
-    const float inv = total_s == 0.f ? 0.f : 1.0f / total_s;
-    const int t = row_of(a, c);
-    uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs + (long)(head * a.group + c - t * a.group) * a.out.hs + d;
-    *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 
 }  // namespace apus
@@ -913,7 +926,8 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     if (a.whole) return 0;
     // the joining kernel starts while the first drains, and waits for it
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.group * a.v.max_rows, a.v.heads, a.v.nseq);
+    // (a block a column, up to 64: max_rows may be far above the rows that there are)
+    cfg.gridDim = dim3((unsigned)std::min((long)a.group * a.v.max_rows, 64l), a.v.heads, a.v.nseq);
     cfg.blockDim = dim3(128);
     cfg.dynamicSmemBytes = (KJ_RUNS + (128 / (D / 4)) * D) * 4;
     cfg.stream = st;

@@ -193,12 +193,15 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                      ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // warp 0: 32 sequences from c0 on, a lane's with its blocks of rows; `before`: blocks before them
-    PromptSeq cs{0, 0, 0, 0};
+    // warp 0: the blocks of rows of 128 sequences from c0 on, four a lane; `before`:
+    // blocks before them
     int c0 = 0, before = 0, cw = 0, cincl = 0;
+    auto blocks_of = [&](int s) { return s < a.nseq ? (prompt_seq(a, s, true).n + C::ROWS - 1) / C::ROWS : 0; };
     auto chunk = [&]() {
-        cs = c0 + lane < a.nseq ? prompt_seq(a, c0 + lane, true) : PromptSeq{0, 0, 0, 0};
-        cw = cincl = (cs.n + C::ROWS - 1) / C::ROWS;
+        cw = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) cw += blocks_of(c0 + 4 * lane + u);
+        cincl = cw;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, cincl, off);
@@ -271,9 +274,9 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             const int head = (int)(idx % (unsigned)a.heads), block = (int)(idx / (unsigned)a.heads);
             if (block < before) { c0 = before = 0; chunk(); }
             int sum = __shfl_sync(0xffffffffu, cincl, 31);
-            while (block >= before + sum && c0 + 32 < a.nseq) {
+            while (block >= before + sum && c0 + 128 < a.nseq) {
                 before += sum;
-                c0 += 32;
+                c0 += 128;
                 chunk();
                 sum = __shfl_sync(0xffffffffu, cincl, 31);
             }
@@ -281,12 +284,23 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             if (block < before + sum) {
                 const int rel = block - before;
                 const int src = __ffs(__ballot_sync(0xffffffffu, cincl - cw <= rel && rel < cincl)) - 1;
+                // the sequence among the lane's four, and the block in it
+                int s = c0 + 4 * lane, left = rel - (cincl - cw);
+                PromptSeq sq{0, 0, 0, 0};
+                if (lane == src)
+#pragma unroll 1
+                    for (int u = 0; u < 4; u++, s++) {
+                        sq = prompt_seq(a, s, false);
+                        const int w = (sq.n + C::ROWS - 1) / C::ROWS;
+                        if (left < w) { left = w - 1 - left; break; }
+                        left -= w;
+                    }
                 PaItem it;
-                it.q0 = __shfl_sync(0xffffffffu, cs.q0, src);
-                it.n = __shfl_sync(0xffffffffu, cs.n, src);
-                it.k0 = __shfl_sync(0xffffffffu, cs.k0, src);
-                it.m = __shfl_sync(0xffffffffu, cs.m, src);
-                it.r0 = (__shfl_sync(0xffffffffu, cincl, src) - 1 - rel) * C::ROWS;
+                it.q0 = __shfl_sync(0xffffffffu, sq.q0, src);
+                it.n = __shfl_sync(0xffffffffu, sq.n, src);
+                it.k0 = __shfl_sync(0xffffffffu, sq.k0, src);
+                it.m = __shfl_sync(0xffffffffu, sq.m, src);
+                it.r0 = __shfl_sync(0xffffffffu, left, src) * C::ROWS;
                 it.head = head;
                 it.first = idx == 0;
                 publish(it);
@@ -456,7 +470,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             // sequences out of bounds behind the last one with rows are reported too
             if (it.first)
 #pragma unroll 4
-                for (int s = 32 + lane; s < a.nseq; s += 32) prompt_seq(a, s, true);
+                for (int s = 128 + lane; s < a.nseq; s += 32) prompt_seq(a, s, true);
             uint32_t *const bad_key = first_bad[k & 1];
             for (int i = lane; i < D; i += 32) bad_key[i] = 0x3fffffffu;
             if (lane == 0) poison[k & 1] = 0;

@@ -17,7 +17,8 @@
  *   - What the host cannot see is checked on the device: a page id, a length
  *     or a row range that is out of bounds is never followed.  It is left out
  *     (below, at each entry) and reported by apus_gcuda_kernel_error():
- *     41 page id, 42 length or row range.
+ *     41 page id, 42 length or row range (43: a wait inside a kernel gave up,
+ *     and that call's outputs are incomplete).
  */
 #ifndef APUS_ATTN_GCUDA_H
 #define APUS_ATTN_GCUDA_H
@@ -114,14 +115,20 @@ int apus_gcuda_kv4_read_dev(const ApusKv4Cache *cache, const ApusKv4Batch *batch
  * sel[r * sel_stride + j / pool] != 0 (0 beyond sel_stride), and always the
  * positions of its own last, incomplete pool.
  *
- * Scores, softmax statistics and sums are fp32; the weights, times the value
- * scales, are rounded to BF16 for the tensor cores.  A row that sees nothing
- * gives zeros, as does a row of a page whose id is out of range (its positions
- * count as unseen).  What stands at unseen positions has no influence, NaN and
- * infinities included.  Rows behind cu_rows[nseq] are left as they are.
- * workspace: 16-byte aligned, at least
- * apus_gcuda_kv4_attn_workspace bytes (0: none needed), private to the call
- * until it has run; its contents need no initialisation. */
+ * Scores, softmax statistics and sums are fp32; a weight is rounded to f16 as
+ * it is and once more times its value's scale, for the tensor cores (2^-11
+ * each; a power of two a position keeps both in f16's range, and what is below
+ * 2^-30 of a row's largest term may add nothing).  Positions in a page whose id
+ * is out of range count as unseen; a row that sees nothing gives zeros.  What
+ * stands at unseen positions has no influence, NaN and infinities included; a
+ * NaN or an infinity in a query row makes that row NaN, and a group of values
+ * that holds NaN those dims of every row that sees it.  Rows behind
+ * cu_rows[nseq] are left as they are.
+ * workspace: 16-byte aligned, at least apus_gcuda_kv4_attn_workspace bytes (0:
+ * none needed, or bad arguments: apus_gcuda_last_error() tells), private to the
+ * call until it has run; its contents need no initialisation.  The bytes go by
+ * the batch's bounds (nseq, max_rows, max_len) and grow with each, so one
+ * workspace for the largest serves all. */
 size_t apus_gcuda_kv4_attn_workspace(const ApusKv4Cache *cache, const ApusKv4Batch *batch, size_t q_heads);
 int apus_gcuda_kv4_attn_dev(const ApusKv4Cache *cache, const ApusKv4Batch *batch, const ApusHeadRows *q,
                             const ApusHeadRows *out, float scale, const uint8_t *sel, size_t sel_stride, size_t pool,

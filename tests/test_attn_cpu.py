@@ -142,6 +142,19 @@ def test_nothing_to_do():
     assert G.apus_gcuda_last_error() == b""
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_workspace_grows_with_the_bounds(dim):
+    for nseq in (1, 2, 48, 300):
+        for max_rows in (1, 2, 3, 4, 5, 17):
+            for max_len in (1, 512, 513, 700, 5000, 131072):
+                def need(n, r, m):
+                    return G.apus_gcuda_kv4_attn_workspace(cache(heads=8, dim=dim), batch(nseq=n, max_rows=r, max_len=m,
+                                                                                          table_stride=4096), 32)
+                at = need(nseq, max_rows, max_len)
+                assert all(need(*b) >= at for b in ((nseq + 1, max_rows, max_len), (nseq, max_rows + 1, max_len),
+                                                    (nseq, max_rows, max_len + 1), (nseq, max_rows, max_len * 2)))
+
+
 def test_page_bytes():
     for heads, dim in ((1, 64), (8, 128), (64, 256)):
         assert G.apus_gcuda_kv4_page_bytes(heads, dim) == heads * 72 * dim

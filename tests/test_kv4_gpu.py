@@ -474,3 +474,35 @@ def test_many_sequences(gcuda, nseq, longest):
     c.fill_all()
     q = bf16(c.g, c.total, 2, 64, std=2.0).cuda()
     c.check(q, c.attn(q, 0.125), 0.125)
+
+
+def test_bound_far_above_the_rows(gcuda):
+    """max_rows far above the rows that there are, and more columns than the joining kernel has blocks."""
+    c = Case(gcuda, 128, 2, [2500, 700, 4000], [3, 40, 1], seed=21, max_rows=5000)
+    c.fill_all()
+    q = bf16(c.g, c.total, 8, 128, std=2.0).cuda()
+    c.check(q, c.attn(q, 0.09), 0.09)
+
+
+@pytest.mark.parametrize("dim,pool,kept", [(64, 4, 0.3), (128, 100, 0.9), (64, 1, 0.02)])
+def test_selected_long(gcuda, dim, pool, kept):
+    """More kept positions than one list holds, and a longer way between them than its offsets reach."""
+    c = Case(gcuda, dim, 1, [150001], [2], seed=pool)
+    c.fill_all()
+    q = bf16(c.g, 2, 2, dim, std=2.0).cuda()
+    sel = (torch.rand(2, 150001 // pool + 1, generator=c.g) < kept).to(torch.uint8)
+    sel[:, 20000 // pool:100000 // pool] = 0
+    sel[1, 90000 // pool] = 1
+    c.check(q, c.attn(q, 0.1, sel.cuda(), pool), 0.1, sel, pool)
+
+
+@pytest.mark.parametrize("length", [100, 6000])
+def test_seen_nan_with_no_weight(gcuda, length):
+    """A value that is NaN reaches the rows that see it however small its weight, in a run of its own too."""
+    c = Case(gcuda, 64, 1, [length], [1], seed=22)
+    k, v = bf16(c.g, length, 1, 64), bf16(c.g, length, 1, 64)
+    q = torch.ones(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    k[10], v[10, 0, 3] = -1000.0, float("nan")
+    c.write_all(k, v)
+    got = c.attn(q, 1.0)
+    assert got[0, 0, :32].isnan().all() and got[0, 0, 32:].isfinite().all()

@@ -154,6 +154,28 @@ def test_many_items(gcuda, dim, heads, group):
         assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
 
 
+@pytest.mark.parametrize("dim", [64, 256])
+def test_many_sequences(gcuda, dim):
+    """More sequences than are looked up at a time, most of a few rows, some empty; a range out of bounds behind the
+    last row is reported."""
+    g = torch.Generator().manual_seed(dim + 2)
+    rows = [int(x) for x in torch.randint(0, 4, (700,), generator=g)]
+    rows[130], rows[500] = 300, 513
+    rows[600:] = [0] * 100
+    q = bf16(g, sum(rows) + 1, 2, dim).cuda()
+    k, v = (bf16(g, sum(rows), 1, dim).cuda() for _ in range(2))
+    out = run(gcuda, q, k, v, rows, rows, 0.1)
+    check(q, k, v, out, rows, rows, 0.1)
+    assert (out[sum(rows):] == 7).all()
+    cu, bad = starts(rows).cuda(), starts(rows).cuda()
+    bad[700] = 1 << 30
+    again = torch.full_like(q, 7.0)
+    gcuda.prompt_attn(gcuda.PromptBatch(bad, cu, max_rows=513), q, k, v, again, 0.1)
+    torch.cuda.synchronize()
+    assert gcuda.apus_gcuda_kernel_error() == 42
+    assert torch.equal(again, out)
+
+
 def test_ranges_out_of_bounds(gcuda):
     g = torch.Generator().manual_seed(10)
     q, k, v = (bf16(g, 100, 2, 64).cuda() for _ in range(3))
