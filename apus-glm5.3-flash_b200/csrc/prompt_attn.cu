@@ -109,20 +109,6 @@ APUS_DEV uint32_t pa_pack(float lo, float hi) {
     return d;
 }
 
-// Whole-warp forms: one elected lane acts, the operands stay in uniform registers.
-APUS_DEV void tma_load_3d_warp(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
-    asm volatile(
-        "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-        " @e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4}], [%5];\n}"
-        ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-APUS_DEV void expect_tx_warp(uint64_t *bar, uint32_t bytes) {
-    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-                 " @e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-
 // A bounded wait.
 APUS_DEV bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *ab) {
     return mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
@@ -307,7 +293,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 const int ntmax = __shfl_sync(0xffffffffu, pa_tiles<NQ>(it).ntmax, 0), khead = head / a.group, entries = 2 * ntmax;
                 const int k_row = it.k0, q_row = it.q0 + it.r0;
                 auto load_q = [&](int part) {
-                    expect_tx_warp(&q_full[part], NQ * C::STAGE);
+                    mbar_arrive_expect_tx_warp(&q_full[part], NQ * C::STAGE);
                     for (int i = 0; i < NQ; i++)
                         for (int p = part * (C::SPAN / 64); p < (part + 1) * (C::SPAN / 64); p++)
                             tma_load_3d_warp(qs + i * C::QTILE + p * pa::PANEL, &qmap, p * 64, head, q_row + i * pa::BM, &q_full[part]);
@@ -321,7 +307,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                         const unsigned s = g % NST;
                         if (g >= NST) wait(&empty[s], (g / NST - 1) & 1);
                         if (!ok) break;
-                        expect_tx_warp(&full[s], C::STAGE);
+                        mbar_arrive_expect_tx_warp(&full[s], C::STAGE);
                         uint8_t *st = ring + s * C::STAGE;
 #pragma unroll
                         for (int p = 0; p < C::SPAN / 64; p++)
