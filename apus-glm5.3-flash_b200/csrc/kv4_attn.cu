@@ -37,7 +37,8 @@
 // Work: a segment is one sequence's positions for one cache head and 8 NT
 // columns.  All segments' pages in a row are cut into equal runs, one a CTA,
 // one wave of CTAs (lengths are read on the device, so ragged batches balance
-// too); a segment that a cut divides is put together by a second kernel.
+// too), or, of few segments, each into runs of its own; a segment that a cut
+// divides is put together by a second kernel.
 // Inside a CTA four warps each stream units of U positions of their own
 // through two stages of their own with their own maximum, sum and output
 // tile, so the loop has no CTA barrier; the warps are joined once a segment.
@@ -48,13 +49,13 @@
 // what no column keeps is neither read nor computed.
 //
 // Measured (us a call; bytes that it has to read, of 6.55 TB/s): one sequence of
-// 131072 positions, 64 heads over 8 of 128: 48 (48%); 48 sequences of up to 8192,
-// 32 over 8: 69 (55%); 4 rows over 4363 positions of 64 heads of 256: 33 (38%);
-// 4 rows of 512 pools of 4 out of 32771: 46.  What bounds it is issue: 330
-// instructions for 16 positions of dim 128 (70 of them LOP3 and 20 shifts at half
-// rate: 48% of that pipe, 59% of all issue slots), and about 8 thousand cycles a
-// launch before and after the stream.  A fourth CTA an SM (128 registers, the
-// query in shared memory) took 8% longer.
+// 131072 positions, 64 heads over 8 of 128: 43 (54%); 48 sequences of up to 8192,
+// 32 over 8: 71 (53%); 4 rows over 4363 positions of 64 heads of 256: 32 (38%);
+// 4 rows of 512 pools of 4 out of 32771: 45; 513 positions, 32 over 8: 8.5.  What
+// bounds it is issue: 330 instructions for 16 positions of dim 128 (70 of them LOP3
+// and 20 shifts at half rate: 48% of that pipe, 59% of all issue slots), and about
+// 8 thousand cycles a launch before and after the stream.  A fourth CTA an SM (128
+// registers, the query in shared memory) took 8% longer.
 #include <algorithm>
 #include <type_traits>
 
@@ -103,7 +104,8 @@ struct Kv4AttnArgs {
     uint64_t pool_magic;      // ceil(2^36 / pool): j / pool = j * magic >> 36 for j < 2^28, pool <= 128
     int whole;                // no segment is cut: a page of work stands for a segment
     int min_pages;            // pages of a run at least
-    long *plan;               // workspace: runs, pages in all, first page of each sequence
+    int slots, segs;          // CTAs that run at once; segments at most
+    long *plan;               // workspace: runs, units of work in all, pages of a unit, first unit of each sequence
     float *part;              // workspace: two partial results a CTA
 };
 
@@ -117,14 +119,15 @@ APUS_DEV int pool_of(const Kv4AttnArgs &a, int j) { return (int)(((uint64_t)(uin
 
 constexpr int KJ_RUNS = 148 * 4;          // runs at most (a multiple of 4)
 
-// The work: sequence s has heads * ncb segments of `pages` pages (one at
-// least, so that a row that sees nothing is written too).
-struct Kv4Work { Kv4Seq sq; int ncb; long pages; };
-APUS_DEV Kv4Work kv4_work(const Kv4AttnArgs &a, int s, int cols_block) {
+// The work: sequence s has heads * ncb segments of `units` units of `unit`
+// pages (one at least, so that a row that sees nothing is written too).
+struct Kv4Work { Kv4Seq sq; int ncb; long units; };
+APUS_DEV Kv4Work kv4_work(const Kv4AttnArgs &a, int s, int cols_block, int unit) {
     Kv4Work w;
     w.sq = kv4_seq(a.v.cu[s], a.v.cu[s + 1], a.v.len[s], a.v.rows, a.v.max_rows, a.v.max_len);
     w.ncb = (w.sq.n * a.group + cols_block - 1) / cols_block;
-    w.pages = a.whole ? 1 : max(1, (w.sq.len + KV4_PAGE - 1) / KV4_PAGE);
+    const int pages = max(1, (w.sq.len + KV4_PAGE - 1) / KV4_PAGE);
+    w.units = a.whole ? 1 : unit == 1 ? pages : (int)((uint32_t)(pages + unit - 1) / (uint32_t)unit);
     return w;
 }
 
@@ -234,17 +237,22 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     __shared__ long found_s[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
 
-    // ---- this CTA's run of pages [x, xe)
+    // ---- this CTA's run of units [x, xe)
     pdl_launch_dependents();
     // weights of the sequences, THREADS at a time: this thread's, the pages
     // before it and (through `before`) those of all
-    auto scan = [&](int s0, long &w, long &before) -> long {
+    int unit = 1, per_unit = 0, pages = 0;      // (this thread's sequence: segments, pages of one)
+    auto scan = [&](int s0, long &w, long &before, bool again) -> long {
         const int s = s0 + threadIdx.x;
         w = 0;
         if (s < a.v.nseq) {
-            const Kv4Work k = kv4_work(a, s, COLS);
-            if (k.sq.bad && blockIdx.x == 0) atomicExch(&g_kv4a_err, (int)ATTN_ERR_SEQ);
-            w = (long)a.v.heads * k.ncb * k.pages;
+            if (!again) {
+                const Kv4Work k = kv4_work(a, s, COLS, 1);
+                if (k.sq.bad && blockIdx.x == 0) atomicExch(&g_kv4a_err, (int)ATTN_ERR_SEQ);
+                per_unit = a.v.heads * k.ncb;
+                pages = (int)k.units;
+            }
+            w = (long)per_unit * (unit == 1 ? pages : (int)((uint32_t)(pages + unit - 1) / (uint32_t)unit));
         }
         long incl = w;
 #pragma unroll
@@ -262,21 +270,34 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         __syncthreads();
         return at;
     };
-    long total = 0, w0 = 0, at0 = 0;
-    for (int s0 = 0; s0 < a.v.nseq; s0 += kv4::THREADS) at0 = scan(s0, w0, total);
-    const long runs = min((long)gridDim.x, max(1l, div_long(total, a.min_pages)));
+    // Runs that end with their segments, where these are few: with `unit` pages a
+    // run, there are at most total / unit + segs of them.  A run across a border has
+    // two pieces to set up and join, which takes as long as 1.5 pages (513 positions,
+    // 8 segments: 10.1 us, and 8.4 with runs of their own).
+    long total, w0 = 0, at0 = 0;
+#pragma unroll 1
+    for (bool again = false;; again = true) {
+        total = 0;
+#pragma unroll 1
+        for (int s0 = 0; s0 < a.v.nseq; s0 += kv4::THREADS) at0 = scan(s0, w0, total, again && a.v.nseq <= kv4::THREADS);
+        if (again || a.whole || a.segs >= a.slots) break;
+        const long u = max((long)a.min_pages, div_long(total + a.slots - a.segs - 1, a.slots - a.segs));
+        if (u != a.min_pages && 2 * u * a.slots > 2 * total + 3 * a.slots) break;
+        unit = (int)u;
+    }
+    const long runs = min((long)gridDim.x, max(1l, unit > 1 ? total : div_long(total, a.min_pages)));
     if (blockIdx.x >= runs && blockIdx.x != 0) return;
     long x = div_long(total * blockIdx.x, runs);
     const long xe = div_long(total * (blockIdx.x + 1), runs);
-    // the sequence in which it begins, and that sequence's first page
+    // the sequence in which it begins, and that sequence's first unit
     long before = 0;
     for (int s0 = 0; s0 < a.v.nseq; s0 += kv4::THREADS) {
-        if (a.v.nseq > kv4::THREADS) at0 = scan(s0, w0, before);
+        if (a.v.nseq > kv4::THREADS) at0 = scan(s0, w0, before, false);
         const int s = s0 + threadIdx.x;
         if (s < a.v.nseq && w0 && at0 <= x && x < at0 + w0) { found_s[0] = s; found_s[1] = at0; }
-        if (blockIdx.x == 0 && a.plan && s < a.v.nseq) a.plan[2 + s] = at0;
+        if (blockIdx.x == 0 && a.plan && s < a.v.nseq) a.plan[3 + s] = at0;
     }
-    if (blockIdx.x == 0 && a.plan && threadIdx.x == 0) { a.plan[0] = runs; a.plan[1] = total; }
+    if (blockIdx.x == 0 && a.plan && threadIdx.x == 0) { a.plan[0] = runs; a.plan[1] = total; a.plan[2] = unit; }
     if (x >= xe) return;
     __syncthreads();
     int seq = (int)found_s[0];
@@ -286,25 +307,25 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     __shared__ int wcount[kv4::WARPS];
 
     while (x < xe) {
-    // ---- the next piece: pages pg0 .. pg1 of one segment
-    Kv4Work wk = kv4_work(a, seq, COLS);
-    while (x >= seq_x + (long)a.v.heads * wk.ncb * wk.pages) {
-        seq_x += (long)a.v.heads * wk.ncb * wk.pages;
-        wk = kv4_work(a, ++seq, COLS);
+    // ---- the next piece: units of one segment
+    Kv4Work wk = kv4_work(a, seq, COLS, unit);
+    while (x >= seq_x + (long)a.v.heads * wk.ncb * wk.units) {
+        seq_x += (long)a.v.heads * wk.ncb * wk.units;
+        wk = kv4_work(a, ++seq, COLS, unit);
     }
     const Kv4Seq sq = wk.sq;
-    const int seg = (int)div_long(x - seq_x, wk.pages);
-    const long seg_x = seq_x + seg * wk.pages;
+    const int seg = (int)div_long(x - seq_x, wk.units);
+    const long seg_x = seq_x + seg * wk.units;
     const int head = wk.ncb == 1 ? seg : seg / wk.ncb, cb = seg - head * wk.ncb;
-    const long piece_e = min(xe, seg_x + wk.pages);
-    const bool starts = x == seg_x, ends = piece_e == seg_x + wk.pages;
+    const long piece_e = min(xe, seg_x + wk.units);
+    const bool starts = x == seg_x, ends = piece_e == seg_x + wk.units;
     const int cols = sq.n * a.group, c0 = cb * COLS;
     const int cend = min(c0 + COLS, cols);
     // the positions that the first and the last row of the block see
     const int lim_row0 = sq.len - sq.n + 1;
     const int lim0 = lim_row0 + row_of(a, c0), lim1 = lim_row0 + row_of(a, cend - 1);
-    const int p0 = a.whole ? 0 : (int)(x - seg_x) * KV4_PAGE;
-    const int p1 = a.whole ? lim1 : min((int)(piece_e - seg_x) * KV4_PAGE, lim1);
+    const int p0 = a.whole ? 0 : (int)(x - seg_x) * unit * KV4_PAGE;
+    const int p1 = a.whole ? lim1 : (int)min((piece_e - seg_x) * unit * KV4_PAGE, (long)lim1);
     const int32_t *table = a.v.table + (long)seq * a.v.table_stride;
 
     // the query rows of this lane's columns, on their way while the first units are fetched
@@ -809,32 +830,46 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
 }
 
 // Joins the pieces of one column of a segment that was cut: weights
-// 2^(m_c - max m), in the order of the runs.
-template <int D>
-__global__ void __launch_bounds__(128) k_kv4_join(const Kv4AttnArgs a, int cols_block) {
-    constexpr int L = D / 4, P = 128 / L;      // lanes over the dims, parts over the pieces
-    extern __shared__ float kj_dyn[];          // weights of the pieces, then [P][D] sums
+// 2^(m_c - max m), in the order of the runs.  What it reads is on its way
+// together: each thread's first AHEAD pieces before the weights are known.
+// Two forms (kv4_attn_launch): WIDE for few columns, which may be cut into many
+// pieces; the other for many, of few pieces each.
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(const Kv4AttnArgs a, int cols_block) {
+    constexpr int L = D / 4, P = (WIDE ? 256 : 128) / L, AHEAD = WIDE ? 8 : 1;
+        // lanes over the dims, parts over the pieces
+    extern __shared__ float kj_dyn[];                 // weights of the pieces, then [P][D] sums
     __shared__ float total_s;
     const int seq = blockIdx.z, head = blockIdx.y;
-    const Kv4Work wk = kv4_work(a, seq, cols_block);
+    Kv4Work wk = kv4_work(a, seq, cols_block, 1);
     const Kv4Seq sq = wk.sq;
-    pdl_wait();                                // the partial results and the plan
+    pdl_wait();                                       // the partial results and the plan
+    const long runs = a.plan[0], total = a.plan[1], first = a.plan[3 + seq];
+    const int unit = (int)a.plan[2];
+    if (unit > 1) wk.units = (uint32_t)((int)wk.units + unit - 1) / (uint32_t)unit;
     for (int c = blockIdx.x; c < sq.n * a.group; c += gridDim.x) {
         const int cb = c / cols_block, cc = c % cols_block;
-        const long runs = a.plan[0], total = a.plan[1];
-        const long b = a.plan[2 + seq] + ((long)head * wk.ncb + cb) * wk.pages, e = b + wk.pages;
-        const long i0 = ((b + 1) * runs - 1) / total, i1 = (e * runs - 1) / total;   // runs of the first and the last page
-        if (i0 == i1) continue;                    // written by its only run
-        const int n = (int)(i1 - i0) + 1;
-        const size_t stride = (size_t)cols_block * (D + 2);
-        auto piece = [&](int i) { return a.part + ((size_t)(i0 + i) * 2 + (i == 0 ? 1 : 0)) * stride; };
-        float *sums = kj_dyn + KJ_RUNS;
+        const long b = first + ((long)head * wk.ncb + cb) * wk.units, e = b + wk.units;
+        // runs of the first and the last unit
+        const long i0 = runs == total ? b : div_long((b + 1) * runs - 1, total);
+        const long i1 = runs == total ? e - 1 : div_long(e * runs - 1, total);
+        if (i0 == i1) continue;                       // written by its only run
+        const int n = (int)(i1 - i0) + 1, stride = cols_block * (D + 2);
+        const float *const parts = a.part + (size_t)i0 * 2 * (size_t)stride;
+        auto piece = [&](int i) { return parts + (size_t)(2 * i + (i == 0 ? 1 : 0)) * (size_t)stride; };
+        const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L, at = 2 * cols_block + cc * D + d;
+        float4 y[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+            y[u] = part + u * P < n ? *(const float4 *)(piece(part + u * P) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
         if (threadIdx.x < 32) {
             float mx = kv4::NEG_INF;
+#pragma unroll 4
             for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, piece(i)[cc]);
 #pragma unroll
             for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             float sum = 0.f;
+#pragma unroll 4
             for (int i = threadIdx.x; i < n; i += 32) {
                 const float mi = piece(i)[cc], li = piece(i)[cols_block + cc];
                 const float k = mi == kv4::NEG_INF && li == 0.f ? 0.f : ex2(mi - mx);
@@ -846,28 +881,25 @@ __global__ void __launch_bounds__(128) k_kv4_join(const Kv4AttnArgs a, int cols_
             if (threadIdx.x == 0) total_s = sum;
         }
         __syncthreads();
-        const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](const float4 &x, float k) { o.x += x.x * k; o.y += x.y * k; o.z += x.z * k; o.w += x.w * k; };
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+            if (part + u * P < n) add(y[u], kj_dyn[part + u * P]);
 #pragma unroll 4
-        for (int i = part; i < n; i += P) {
-            const float k = kj_dyn[i];
-            const float4 y = *(const float4 *)(piece(i) + 2 * cols_block + cc * D + d);
-            o.x += y.x * k; o.y += y.y * k; o.z += y.z * k; o.w += y.w * k;
-        }
+        for (int i = part + AHEAD * P; i < n; i += P) add(*(const float4 *)(piece(i) + at), kj_dyn[i]);
+        float *const sums = kj_dyn + KJ_RUNS;
         *(float4 *)(sums + part * D + d) = o;
         __syncthreads();
         if (part == 0) {
 #pragma unroll
-            for (int i = 1; i < P; i++) {
-                const float4 y = *(const float4 *)(sums + i * D + d);
-                o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
-            }
+            for (int i = 1; i < P; i++) add(*(const float4 *)(sums + i * D + d), 1.0f);
             const float inv = total_s == 0.f ? 0.f : 1.0f / total_s;
             const int t = row_of(a, c);
             uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs + (long)(head * a.group + c - t * a.group) * a.out.hs + d;
             *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
         }
-        __syncthreads();                           // the next column's weights and sums
+        __syncthreads();                              // the next column's weights and sums
     }
 }
 
@@ -879,7 +911,7 @@ namespace {
 // How a batch is cut: columns of a block, CTAs, whether segments stay whole.
 constexpr long MAX_POS = 1l << 28;
 constexpr long WHOLE_PAGES = 8, MIN_PAGES = 2;
-struct Kv4Plan { int nt, grid, whole; size_t plan_bytes, bytes; };
+struct Kv4Plan { int nt, grid, whole, slots, segs; size_t plan_bytes, bytes; };
 
 Kv4Plan kv4_plan(const Kv4View &v, size_t q_heads) {
     Kv4Plan p;
@@ -888,9 +920,11 @@ Kv4Plan kv4_plan(const Kv4View &v, size_t q_heads) {
     const long pages = v.max_len > KV4_PAGE ? (v.max_len + KV4_PAGE - 1) / KV4_PAGE : 1;
     const long segs = (long)v.nseq * v.heads * ((cols + 8 * p.nt - 1) / (8 * p.nt));
     p.whole = pages <= WHOLE_PAGES;
-    const long most = p.whole ? segs : (segs * pages + MIN_PAGES - 1) / MIN_PAGES, slots = 148 * kv4::resident(p.nt);
-    p.grid = (int)(most < slots ? most : slots);
-    p.plan_bytes = ((size_t)v.nseq + 2) * sizeof(long);
+    const long most = p.whole ? segs : segs * ((pages + MIN_PAGES - 1) / MIN_PAGES);
+    p.slots = 148 * kv4::resident(p.nt);
+    p.segs = (int)(segs < p.slots ? segs : p.slots);
+    p.grid = (int)(most < p.slots ? most : p.slots);
+    p.plan_bytes = ((size_t)v.nseq + 3) * sizeof(long);
     p.plan_bytes = (p.plan_bytes + 15) / 16 * 16;
     p.bytes = p.whole ? 0 : p.plan_bytes + (size_t)p.grid * 2 * (8 * p.nt) * (v.dim + 2) * sizeof(float);
     return p;
@@ -924,19 +958,24 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     k_kv4_attn<D, NT, SEL><<<grid, kv4::THREADS, smem, st>>>(a);
     if (gcuda_check(cudaGetLastError(), "kv4_attn launch")) return -1;
     if (a.whole) return 0;
-    // the joining kernel starts while the first drains, and waits for it
+    // the joining kernel starts while the first drains, and waits for it: a block a
+    // column, up to 64 (max_rows may be far above the rows that there are).  The wide
+    // form where all blocks are resident at once (131072 positions, 8 segments: 43 us,
+    // 47 with the other; 48 sequences, 384 segments: 69 us, 79 with the wide form).
+    const long bx = std::min((long)a.group * a.v.max_rows, 64l);
+    const bool wide = bx * a.v.heads * a.v.nseq <= 2 * 148;
     cudaLaunchConfig_t cfg{};
-    // (a block a column, up to 64: max_rows may be far above the rows that there are)
-    cfg.gridDim = dim3((unsigned)std::min((long)a.group * a.v.max_rows, 64l), a.v.heads, a.v.nseq);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = (KJ_RUNS + (128 / (D / 4)) * D) * 4;
+    cfg.gridDim = dim3((unsigned)bx, a.v.heads, a.v.nseq);
+    cfg.blockDim = dim3(wide ? 256 : 128);
+    cfg.dynamicSmemBytes = (KJ_RUNS + (wide ? 256 : 128) * 4) * 4;
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    return gcuda_check(cudaLaunchKernelEx(&cfg, k_kv4_join<D>, a, 8 * NT), "kv4_attn join launch");
+    return gcuda_check(cudaLaunchKernelEx(&cfg, wide ? k_kv4_join<D, true> : k_kv4_join<D, false>, a, 8 * NT),
+                       "kv4_attn join launch");
 }
 template <int D, int NT> int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     return a.sel ? kv4_attn_launch<D, NT, true>(a, grid, st) : kv4_attn_launch<D, NT, false>(a, grid, st);
@@ -985,6 +1024,8 @@ extern "C" int apus_gcuda_kv4_attn_dev(const ApusKv4Cache *cache, const ApusKv4B
     a.pool_magic = (((uint64_t)1 << 36) + (uint64_t)a.pool - 1) / (uint64_t)a.pool;
     a.whole = p.whole;
     a.min_pages = p.whole ? 1 : (int)MIN_PAGES;
+    a.slots = p.slots;
+    a.segs = p.segs;
     a.plan = p.whole ? nullptr : (long *)workspace;
     a.part = p.whole ? nullptr : (float *)((char *)workspace + p.plan_bytes);
     cudaStream_t st = (cudaStream_t)stream;
