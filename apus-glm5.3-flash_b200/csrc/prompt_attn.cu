@@ -36,12 +36,13 @@
 // (clusterlaunchcontrol), so the next item's copies and first products run under
 // the last one's end.  One CTA an item spent 12.7 thousand cycles on set-up, first
 // copies and the end, where 2048 rows of dim 256 take 37 thousand: 172 -> 162 us,
-// seven ragged prompts of dim 128 81 -> 75 us, nine of dim 256 71 -> 62 us.
+// seven ragged prompts of dim 128 81 -> 75 us, nine of dim 256 71 -> 62 us.  Heads
+// that do not fit L2 together follow one another (L2_SHARE): 162 -> 144 us.
 //
 // Measured: dim 128, 8192 rows after 4096 keys, 32 heads over 8: 0.79 ms, 1380
-// TFLOP/s; dim 256, 8192 rows of 16 heads: 1210 TFLOP/s, there bound by the ring,
-// which holds two tiles and no more fit (five half tiles in place of four: 1250;
-// quarters, V by keys, 730; two softmax groups that take turns, 1160).
+// TFLOP/s; dim 256, 8192 rows of 16 heads: 1250 TFLOP/s, 2400 cycles a tile of 2048
+// (a ring of five half tiles in place of four, the same; quarters, V by keys, 730;
+// two softmax groups that take turns, 1160).
 //
 // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value would
 // reach the row through the product.  So in tiles with hidden keys such values
@@ -96,6 +97,11 @@ template <int D> struct Cfg {
                                         ((uint32_t)(SPAN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 };
 constexpr float RAISE = 8.0f;
+// Bytes of keys and values that items next to one another read: all items that
+// run at once read them at their own places, so what does not stay in L2 (126 MB)
+// comes from HBM for each block of rows.  64 heads of 256, 2048 rows: 144 us (all
+// heads together, 134 MB: 165; 64 MB 149, 32 MB 144); 4096 rows: 490 (573).
+constexpr int L2_SHARE = 48 << 20;
 }  // namespace pa
 
 APUS_DEV float pa_ex2(float x) {
@@ -234,8 +240,10 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
     // thread, so the first gives 80 of its up (88 x 128 + 208 x 256 = 168 x 384).
     if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {                    // ---- items and copies
-        // Blocks of ROWS rows in the order of the sequences, a sequence's last block
-        // (the one with the most keys) first; the heads of a block follow one another.
+        // Items in the order of the sequences; in a sequence equal parts of the heads
+        // whose keys and values take up to L2_SHARE bytes, of a part the last block of
+        // ROWS rows (the one with the most keys) first, and the heads of a block one
+        // after the other.
         unsigned idx = blockIdx.x, g = 0, asked = 0;
         int k = 0, loaded = 0;
         bool ok = true;
@@ -257,7 +265,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             k++;
         };
         while (true) {
-            const int head = (int)(idx % (unsigned)a.heads), block = (int)(idx / (unsigned)a.heads);
+            const int block = (int)(idx / (unsigned)a.heads);
             if (block < before) { c0 = before = 0; chunk(); }
             int sum = __shfl_sync(0xffffffffu, cincl, 31);
             while (block >= before + sum && c0 + 128 < a.nseq) {
@@ -270,15 +278,15 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             if (block < before + sum) {
                 const int rel = block - before;
                 const int src = __ffs(__ballot_sync(0xffffffffu, cincl - cw <= rel && rel < cincl)) - 1;
-                // the sequence among the lane's four, and the block in it
-                int s = c0 + 4 * lane, left = rel - (cincl - cw);
+                // the sequence among the lane's four, its first block and their number
+                int s = c0 + 4 * lane, left = rel - (cincl - cw), w = 0;
                 PromptSeq sq{0, 0, 0, 0};
                 if (lane == src)
 #pragma unroll 1
                     for (int u = 0; u < 4; u++, s++) {
                         sq = prompt_seq(a, s, false);
-                        const int w = (sq.n + C::ROWS - 1) / C::ROWS;
-                        if (left < w) { left = w - 1 - left; break; }
+                        w = (sq.n + C::ROWS - 1) / C::ROWS;
+                        if (left < w) break;
                         left -= w;
                     }
                 PaItem it;
@@ -286,7 +294,17 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 it.n = __shfl_sync(0xffffffffu, sq.n, src);
                 it.k0 = __shfl_sync(0xffffffffu, sq.k0, src);
                 it.m = __shfl_sync(0xffffffffu, sq.m, src);
-                it.r0 = __shfl_sync(0xffffffffu, left, src) * C::ROWS;
+                w = __shfl_sync(0xffffffffu, w, src);
+                left = __shfl_sync(0xffffffffu, left, src);
+                // place in the sequence's items -> heads together, block, head
+                const unsigned local = idx - (unsigned)(block - left) * (unsigned)a.heads;
+                const unsigned kheads = (unsigned)(a.heads / a.group);
+                const unsigned fit = max(1u, (unsigned)(pa::L2_SHARE / (4 * D)) / (unsigned)max(it.m, 1));
+                const unsigned parts = (kheads + fit - 1) / fit, share = (kheads + parts - 1) / parts * (unsigned)a.group;
+                const unsigned h0 = local / (share * (unsigned)w) * share, in = local - h0 * (unsigned)w;
+                const unsigned hn = min(share, (unsigned)a.heads - h0), nth = in / hn;
+                const int head = (int)(h0 + (in - nth * hn));
+                it.r0 = (w - 1 - (int)nth) * C::ROWS;
                 it.head = head;
                 it.first = idx == 0;
                 publish(it);

@@ -154,6 +154,16 @@ def test_many_items(gcuda, dim, heads, group):
         assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
 
 
+def test_heads_in_parts(gcuda):
+    """Sequences whose keys and values do not stay in L2 together: their heads are taken in parts, the last one
+    smaller; one before and one behind whose heads are taken together."""
+    g = torch.Generator().manual_seed(14)
+    rows, keys = [40, 300, 129, 70], [50, 6000, 4100, 70]
+    q = bf16(g, sum(rows), 26, 256).cuda()
+    k, v = (bf16(g, sum(keys), 13, 256).cuda() for _ in range(2))
+    check(q, k, v, run(gcuda, q, k, v, rows, keys, 0.07), rows, keys, 0.07)
+
+
 @pytest.mark.parametrize("dim", [64, 256])
 def test_many_sequences(gcuda, dim):
     """More sequences than are looked up at a time, most of a few rows, some empty; a range out of bounds behind the
