@@ -49,13 +49,14 @@
 // what no column keeps is neither read nor computed.
 //
 // Measured (us a call; bytes that it has to read, of 6.55 TB/s): one sequence of
-// 131072 positions, 64 heads over 8 of 128: 43 (54%); 48 sequences of up to 8192,
-// 32 over 8: 71 (53%); 4 rows over 4363 positions of 64 heads of 256: 32 (38%);
+// 131072 positions, 64 heads over 8 of 128: 41.5 (56%); 48 sequences of up to 8192,
+// 32 over 8: 68.5 (55%); 4 rows over 4363 positions of 64 heads of 256: 31 (39%);
 // 4 rows of 512 pools of 4 out of 32771: 45; 513 positions, 32 over 8: 8.5.  What
-// bounds it is issue: 330 instructions for 16 positions of dim 128 (70 of them LOP3
+// bounds it is issue: 322 instructions for 16 positions of dim 128 (70 of them LOP3
 // and 20 shifts at half rate: 48% of that pipe, 59% of all issue slots), and about
 // 8 thousand cycles a launch before and after the stream.  A fourth CTA an SM (128
-// registers, the query in shared memory) took 8% longer.
+// registers, the query in shared memory) took 8% longer; two scores an
+// instruction (packed fp32) took 3% off.
 #include <algorithm>
 #include <type_traits>
 
@@ -418,6 +419,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                 for (int i = 0; i < JB; i++) { wa[h * JB + i] = ta[i]; wb[h * JB + i] = tb[i]; }
             }
             float sa[NG], sb[NG];
+            uint64_t z2[NT][2];
             lds_floats<NG>(sa, (const float *)(own + C::KF) + (at + pg) * NG);
             lds_floats<NG>(sb, (const float *)(own + C::KF) + (at + pg + 8) * NG);
             pw[0] = *(const float2 *)(own + C::PW + (at + pg) * 8);
@@ -433,12 +435,19 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                     else qf = make_uint4(Q[nt][j][0], Q[nt][j][1], Q[nt][j][2], Q[nt][j][3]);
                     mma_f16(c, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, qf.x, qf.y);
                     mma_f16(c, xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, qf.z, qf.w);
+                    const uint64_t off = f32_pair(cinit[nt][j][0], cinit[nt][j][1]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = c[i] + cinit[nt][j][i & 1], s = i < 2 ? sa[j] : sb[j];
-                        z[nt][i] = j ? fmaf(s, x, z[nt][i]) : s * x;
+                    for (int h = 0; h < 2; h++) {
+                        const uint64_t s = h ? f32_pair(sb[j], sb[j]) : f32_pair(sa[j], sa[j]);
+                        const uint64_t x = add_f32x2(f32_pair(c[2 * h], c[2 * h + 1]), off);
+                        z2[nt][h] = j ? fma_f32x2(s, x, z2[nt][h]) : mul_f32x2(s, x);
                     }
                 }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                f32_unpair(z2[nt][0], z[nt][0], z[nt][1]);
+                f32_unpair(z2[nt][1], z[nt][2], z[nt][3]);
             }
         }
         // ---- running maximum of z + E, so of what a position adds to the output:

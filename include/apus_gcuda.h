@@ -38,8 +38,8 @@ int  apus_gcuda_is_enabled(void);                        /* c/backend_gmetal.h:1
 const char *apus_gcuda_last_error(void);
 void apus_gcuda_clear_error(void);
 /* Device-side error word of the pipelined kernels (0 = none; nonzero = a
- * bounded wait gave up: 1 producer, 2 consumer), read and cleared.
- * Synchronises the device. */
+ * bounded wait gave up: 1 producer, 2 consumer; 41-43: the operators of
+ * apus_attn_gcuda.h), read and cleared.  Synchronises the device. */
 int apus_gcuda_kernel_error(void);
 
 /* Persistent HBM residency for a model-owned host weight region: the bytes
