@@ -667,21 +667,17 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
             // 16-byte pieces, swizzled by the row
 #pragma unroll 1
             for (int c = 0; c < D; c += 64) {
-#pragma unroll 1
-                for (int half = 0; half < 2; half++) {
-                    uint32_t o[32];
-                    if (nti > 0) tc_ld32(o_col + c + half * 32, o);
-                    else
+                float o[64];
+                if (nti > 0) tc_ld64(o_col + c, o);
+                else
 #pragma unroll
-                        for (int h = 0; h < 32; h++) o[h] = 0;
+                    for (int h = 0; h < 64; h++) o[h] = 0.f;
 #pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        uint32_t w[4];
+                for (int h = 0; h < 8; h++) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int x = 0; x < 4; x++)
-                            w[x] = pa_pack(__uint_as_float(o[8 * h + 2 * x]) * inv, __uint_as_float(o[8 * h + 2 * x + 1]) * inv);
-                        *(uint4 *)(own + ln * 128 + (((half * 4 + h) ^ (ln & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int x = 0; x < 4; x++) w[x] = pa_pack(o[8 * h + 2 * x] * inv, o[8 * h + 2 * x + 1] * inv);
+                    *(uint4 *)(own + ln * 128 + ((h ^ (ln & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
                 if (bad)
 #pragma unroll 1
@@ -694,10 +690,14 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                         else if ((pos || neg) && (*o & 0x7fff) <= 0x7f80) *o = pos ? 0x7f80 : 0xff80;
                     }
                 __syncwarp();
+                // (a warp's row 4 r + ln / 8, piece ln % 8)
+                uint16_t *to = op + (long)(ln >> 3) * a.out.rs + c + (ln & 7) * 8;
 #pragma unroll
                 for (int r = 0; r < 32; r += 4) {
-                    const int rr = r + (ln >> 3), piece = ln & 7;
-                    if (rr < left) *(uint4 *)(op + (long)rr * a.out.rs + c + piece * 8) = lds128(own + rr * 128 + ((piece ^ (rr & 7)) << 4));
+                    const int rr = r + (ln >> 3);
+                    const uint4 x = lds128(own + rr * 128 + (((ln & 7) ^ (rr & 7)) << 4));
+                    if (rr < left) *(uint4 *)to = x;
+                    to += 4 * a.out.rs;
                 }
                 __syncwarp();
             }
