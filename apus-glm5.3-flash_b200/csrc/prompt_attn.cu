@@ -115,6 +115,13 @@ APUS_DEV uint32_t pa_pack(float lo, float hi) {
     return d;
 }
 
+// acc + 0 x for two BF16.
+APUS_DEV uint32_t pa_times_0(uint32_t x, uint32_t acc) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0u), "r"(acc));
+    return d;
+}
+
 // A bounded wait.
 APUS_DEV bool pa_wait(uint64_t *bar, uint32_t parity, volatile int *ab) {
     return mbar_wait(bar, parity, ab, &g_pa_err, (int)ATTN_ERR_WAIT);
@@ -494,8 +501,8 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                         uint8_t *st = ring + s * C::STAGE;
                         const int key0 = tile * pa::BN;
                         const int behind = it.m - key0;                 // rows from here on belong to no key
-                        // eight 16-byte pieces at a time: an exponent of all ones carries
-                        // into the sign bit
+                        // eight 16-byte pieces at a time: 0 times a NaN or an infinity is NaN
+                        // and stays in the sum, 0 times anything else adds nothing
                         for (int i = lane * 16; i < C::STAGE; i += 8 * 32 * 16) {
                             uint4 w[8];
 #pragma unroll
@@ -508,12 +515,15 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                                         *(uint4 *)(st + i + u * 512) = w[u];
                                     }
                             }
-                            uint32_t bad = 0;
+                            uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
-                            for (int u = 0; u < 8; u++)
-                                bad |= ((w[u].x & 0x7f807f80u) + 0x00800080u) | ((w[u].y & 0x7f807f80u) + 0x00800080u) |
-                                       ((w[u].z & 0x7f807f80u) + 0x00800080u) | ((w[u].w & 0x7f807f80u) + 0x00800080u);
-                            if (!(bad & 0x80008000u)) continue;
+                            for (int u = 0; u < 8; u++) {
+                                sum[0] = pa_times_0(w[u].x, sum[0]);
+                                sum[1] = pa_times_0(w[u].y, sum[1]);
+                                sum[2] = pa_times_0(w[u].z, sum[2]);
+                                sum[3] = pa_times_0(w[u].w, sum[3]);
+                            }
+                            if (!((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu)) continue;
 #pragma unroll 1
                             for (int u = 0; u < 8; u++) {
                                 const int at = i + u * 512, r = (at / 128) & 127;
