@@ -31,6 +31,10 @@
 //   * Scales are unpacked once a unit, not once a lane that needs them: fp32 for
 //     the keys; for the values f16 below 2, with a power of two a position that
 //     goes into the weight's exponent.  Two f16 roundings (2^-11 each) a weight.
+//   * So there are two running maxima: of z + E (2^E a position's power of two)
+//     for the output's weights, and of z alone for their sum, whose exponentials
+//     are computed a second time.  One weight for both, times 2^-E in the sum, lost
+//     a position whose values are zero or 2^127 below the others', or overflowed.
 // (E4M3 mma.sync looks four times as fast but is carried out as conversions and
 // f16 products: 50 conversions for 16 positions of dim 128, and no faster.)
 //
@@ -79,9 +83,9 @@ template <int D> struct Cfg {
     static constexpr int KC = 0, VC = U * D / 2, KS = U * D, VS = KS + U * NG * 2;
     static constexpr int STAGE = VS + U * NG * 2;           // 72 D U / 64
     // a unit's scales as the loop wants them: keys' fp32 [U][NG], values' f16
-    // pairs of positions, and each position's power of two with its inverse
+    // pairs of positions, and each position's exponent E
     static constexpr int KF = STAGES * STAGE, VH = KF + U * NG * 4, PW = VH + U * NG * 2;
-    static constexpr int WARP_SMEM = PW + U * 8;
+    static constexpr int WARP_SMEM = PW + U * 4;
     // the query's fragments, 512 bytes a group: 32 registers at dim 256, which the
     // loop has not (it spilt); below they stay in registers
     static constexpr bool QS = D == 256;
@@ -91,6 +95,11 @@ template <int D> struct Cfg {
 // each row of the block that keeps the position.
 constexpr int LIST = 4096, LIST_SPAN = 65536, LOOK = 4;     // LOOK: pools that a thread looks at together
 constexpr float NEG_INF = -__builtin_huge_valf();
+// A maximum is raised when a term passes it by more than 2^OVER (the output's weights
+// are f16) or 2^L_OVER (the sum is fp32 and has room for 2^67 such terms).
+constexpr float OVER = 13.0f, L_OVER = 60.0f;
+// A partial result: maximum, sum and the sum's maximum of each column, then its dims.
+constexpr int part_floats(int cols, int dim) { return cols * (dim + 3); }
 }  // namespace kv4
 
 struct Kv4AttnArgs {
@@ -158,6 +167,22 @@ APUS_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^e; 0 below the normal range.  The maxima are whole numbers, so that what they
+// rescale is not rounded.  (The difference of two infinities, NaN, counts as 0: it
+// arises where no position is seen, or in rows that are NaN already.)
+APUS_DEV float pow2(int e) { return __int_as_float(max(min(e, 127) + 127, 0) << 23); }
+// o / sum, brought from the output's maximum m to the sum's maximum ml: by two factors,
+// since m - ml goes from -140 to 187 and the result alone has to fit.
+struct Kv4Norm {
+    float inv, a, b;
+    APUS_DEV Kv4Norm(float sum, float m, float ml) {
+        const int d = max(min((int)(m - ml), 250), -250);
+        inv = sum == 0.f ? 0.f : 1.0f / sum;
+        a = pow2(d >> 1);
+        b = pow2(d - (d >> 1));
+    }
+    APUS_DEV float operator()(float o) const { return o * inv * a * b; }
+};
 // 8x8 transpose of f16 pairs across the warp.
 APUS_DEV uint32_t movmatrix(uint32_t a) {
     uint32_t d;
@@ -233,7 +258,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     constexpr int NG = C::NG, U = C::U, COLS = 8 * NT, UPP = KV4_PAGE / U;
     constexpr float NEG_INF = kv4::NEG_INF;
     extern __shared__ __align__(128) uint8_t kv4_dyn[];
-    __shared__ float join_m[kv4::WARPS][COLS], join_l[kv4::WARPS][COLS];
+    __shared__ float join_m[kv4::WARPS][COLS], join_l[kv4::WARPS][COLS], join_ml[kv4::WARPS][COLS];
     __shared__ long scan_s[kv4::WARPS];
     __shared__ long found_s[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
@@ -347,14 +372,16 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     uint32_t Q[C::QS ? 1 : NT][C::QS ? 1 : NG][4];
     float cinit[NT][NG][2], fac[NT][2];
     int lim[NT][2];
-    float O[NT][D / 16][4], m[NT][2], l[NT][2];      // columns 2 q4, 2 q4 + 1; l: this lane's positions
+    // columns 2 q4, 2 q4 + 1: output and its maximum (of z + E), the sum of this lane's
+    // weights and its maximum (of z)
+    float O[NT][D / 16][4], m[NT][2], l[NT][2], ml[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) O[nt][i][e] = 0.f;
-        m[nt][0] = m[nt][1] = NEG_INF;
+        m[nt][0] = m[nt][1] = ml[nt][0] = ml[nt][1] = NEG_INF;
         l[nt][0] = l[nt][1] = 0.f;
     }
 
@@ -388,7 +415,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             e = max(min(e, 120), -112);
             inv[u] = __int_as_float((127 - e) << 23);
             const int r = NG == 2 ? 2 * lane + u : lane / (NG / 4);
-            *(float2 *)(own + C::PW + r * 8) = make_float2((float)e, inv[u]);
+            *(float *)(own + C::PW + r * 4) = (float)e;
         }
         if constexpr (NG > 2) inv[1] = inv[0];
 #pragma unroll
@@ -405,7 +432,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     auto process = [&](const uint8_t *st, int at, int pos0, const uint32_t *names, auto masked_t) {
         constexpr bool MASKED = decltype(masked_t)::value;
         float z[NT][4];                // positions pg (0, 1), pg + 8 (2, 3); columns 2 q4 (0, 2), 2 q4 + 1
-        float2 pw[2];                  // their powers of two
+        float pw[2];                   // their exponents E
         {
             uint32_t wa[NG], wb[NG];
             constexpr int JB = NG < 4 ? NG : 4;
@@ -422,8 +449,8 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             uint64_t z2[NT][2];
             lds_floats<NG>(sa, (const float *)(own + C::KF) + (at + pg) * NG);
             lds_floats<NG>(sb, (const float *)(own + C::KF) + (at + pg + 8) * NG);
-            pw[0] = *(const float2 *)(own + C::PW + (at + pg) * 8);
-            pw[1] = *(const float2 *)(own + C::PW + (at + pg + 8) * 8);
+            pw[0] = *(const float *)(own + C::PW + (at + pg) * 4);
+            pw[1] = *(const float *)(own + C::PW + (at + pg + 8) * 4);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 const uint32_t xa = wa[j] >> 8, xb = wb[j] >> 8;
@@ -446,36 +473,39 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                f32_unpair(z2[nt][0], z[nt][0], z[nt][1]);
-                f32_unpair(z2[nt][1], z[nt][2], z[nt][3]);
+                const uint64_t f = f32_pair(fac[nt][0], fac[nt][1]);
+                f32_unpair(mul_f32x2(z2[nt][0], f), z[nt][0], z[nt][1]);
+                f32_unpair(mul_f32x2(z2[nt][1], f), z[nt][2], z[nt][3]);
             }
         }
         // ---- running maximum of z + E, so of what a position adds to the output:
         // its weight times 2^E, and times a scale below 2, then fits f16 with the
         // largest at 2^5 to 2^13 whatever the scales' range (what is below 2^-30 of
-        // the largest may add nothing).  It is raised only when a score passes it by
-        // more than 2^13.
+        // the largest may add nothing).  That of z, for the sum.
         uint32_t hide = 0;             // bit nt * 4 + i (MASKED)
         bool over = false;
-        float high[NT][2];
+        float ze[NT][4], high[NT][2], high_l[NT][2];
         uint32_t name[2] = {0, 0};
         if (SEL) { name[0] = names[pg]; name[1] = names[pg + 8]; }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
+            if (MASKED) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float v = fmaf(z[nt][i], fac[nt][i & 1], pw[i >> 1].x);
-                if (MASKED) {
+                for (int i = 0; i < 4; i++) {
                     const bool see = SEL ? (name[i >> 1] >> lim[nt][i & 1] & 1) != 0
                                          : pos0 + (i >> 1) * 8 + pg < lim[nt][i & 1];
-                    if (!see) { v = NEG_INF; hide |= 1u << (nt * 4 + i); }
+                    if (!see) { z[nt][i] = NEG_INF; hide |= 1u << (nt * 4 + i); }
                 }
-                z[nt][i] = v;
             }
 #pragma unroll
+            for (int h = 0; h < 2; h++)
+                f32_unpair(add_f32x2(f32_pair(z[nt][2 * h], z[nt][2 * h + 1]), f32_pair(pw[h], pw[h])), ze[nt][2 * h],
+                           ze[nt][2 * h + 1]);
+#pragma unroll
             for (int u = 0; u < 2; u++) {
-                high[nt][u] = fmaxf(z[nt][u], z[nt][u + 2]);
-                over |= high[nt][u] > m[nt][u] + 13.0f;
+                high[nt][u] = fmaxf(ze[nt][u], ze[nt][u + 2]);
+                high_l[nt][u] = fmaxf(z[nt][u], z[nt][u + 2]);
+                over |= high[nt][u] > m[nt][u] + kv4::OVER || high_l[nt][u] > ml[nt][u] + kv4::L_OVER;
             }
         }
         if (__any_sync(0xffffffffu, over)) {
@@ -483,14 +513,21 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    float x = high[nt][u];
+                    float x = high[nt][u], xl = high_l[nt][u];
 #pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                    if (!(x > m[nt][u] + 13.0f)) continue;         // each column by its own scores alone
-                    x -= 5.0f;
-                    const float down = m[nt][u] == NEG_INF ? 0.f : ex2(m[nt][u] - x);
+                    for (int off = 4; off < 32; off <<= 1) {
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+                        xl = fmaxf(xl, __shfl_xor_sync(0xffffffffu, xl, off));
+                    }
+                    if (xl > ml[nt][u] + kv4::L_OVER) {            // each column by its own scores alone
+                        xl = floorf(xl);
+                        l[nt][u] *= pow2((int)(ml[nt][u] - xl));
+                        ml[nt][u] = xl;
+                    }
+                    if (!(x > m[nt][u] + kv4::OVER)) continue;
+                    x = floorf(x) - 5.0f;
+                    const float down = pow2((int)(m[nt][u] - x));
                     m[nt][u] = x;
-                    l[nt][u] *= down;
 #pragma unroll
                     for (int i = 0; i < D / 16; i++) { O[nt][i][u] *= down; O[nt][i][u + 2] *= down; }
                 }
@@ -501,15 +538,24 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float p[4];
+            uint64_t sum = f32_pair(l[nt][0], l[nt][1]);
+            const uint64_t down = f32_pair(-m[nt][0], -m[nt][1]), down_l = f32_pair(-ml[nt][0], -ml[nt][1]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float mm = m[nt][i & 1];
-                p[i] = ex2(z[nt][i] - (MASKED && mm == NEG_INF ? 0.f : mm));
-                // a hidden position's weight is -0: it adds nothing to the sum, and its
-                // sign marks it below, where a NaN scale must not reach the product
-                if (MASKED && (hide >> (nt * 4 + i) & 1)) p[i] = -0.0f;
-                l[nt][i & 1] = fmaf(p[i], pw[i >> 1].y, l[nt][i & 1]);
+            for (int h = 0; h < 2; h++) {
+                float w[2];
+                f32_unpair(add_f32x2(f32_pair(ze[nt][2 * h], ze[nt][2 * h + 1]), down), p[2 * h], p[2 * h + 1]);
+                f32_unpair(add_f32x2(f32_pair(z[nt][2 * h], z[nt][2 * h + 1]), down_l), w[0], w[1]);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    p[2 * h + u] = ex2(p[2 * h + u]);
+                    w[u] = ex2(w[u]);
+                    // a hidden position adds nothing to the sum, and its weight is -0: the sign
+                    // marks it below, where a NaN scale must not reach the product
+                    if (MASKED && (hide >> (nt * 4 + 2 * h + u) & 1)) { p[2 * h + u] = -0.0f; w[u] = 0.f; }
+                }
+                sum = add_f32x2(sum, f32_pair(w[0], w[1]));
             }
+            f32_unpair(sum, l[nt][0], l[nt][1]);
             b0[nt] = movmatrix(pack_f16(p[0], p[1]));
             b1[nt] = movmatrix(pack_f16(p[2], p[3]));
             if (MASKED) {
@@ -789,6 +835,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
             if (g == 0) {
                 join_m[warp][nt * 8 + 2 * q4 + u] = m[nt][u];
                 join_l[warp][nt * 8 + 2 * q4 + u] = l[nt][u];
+                join_ml[warp][nt * 8 + 2 * q4 + u] = ml[nt][u];
             }
         }
     __syncthreads();
@@ -806,31 +853,34 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         }
     __syncthreads();
     const bool last = starts && ends;
-    float *part = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (size_t)(COLS * (D + 2));
+    float *part = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (size_t)kv4::part_floats(COLS, D);
     for (int i = threadIdx.x; i < (cend - c0) * (D / 4); i += kv4::THREADS) {
         const int c = i / (D / 4), d = (i % (D / 4)) * 4;
-        float mx = NEG_INF;
+        float mx = NEG_INF, mxl = NEG_INF;
 #pragma unroll
-        for (int w = 0; w < kv4::WARPS; w++) mx = fmaxf(mx, join_m[w][c]);
+        for (int w = 0; w < kv4::WARPS; w++) {
+            mx = fmaxf(mx, join_m[w][c]);
+            mxl = fmaxf(mxl, join_ml[w][c]);
+        }
         float sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kv4::WARPS; w++) {
-            if (join_m[w][c] == NEG_INF && join_l[w][c] == 0.f) continue;
-            const float k = ex2(join_m[w][c] - mx);
+            if (join_ml[w][c] == NEG_INF && join_l[w][c] == 0.f) continue;
+            const float k = pow2((int)(join_m[w][c] - mx));
             const float4 x = *(const float4 *)(jo + (w * COLS + c) * JD + d);
-            sum += join_l[w][c] * k;
+            sum += join_l[w][c] * pow2((int)(join_ml[w][c] - mxl));
             o.x += x.x * k; o.y += x.y * k; o.z += x.z * k; o.w += x.w * k;
         }
         if (!last) {
-            *(float4 *)(part + 2 * COLS + c * D + d) = o;
-            if (d == 0) { part[c] = mx; part[COLS + c] = sum; }
+            *(float4 *)(part + 3 * COLS + c * D + d) = o;
+            if (d == 0) { part[c] = mx; part[COLS + c] = sum; part[2 * COLS + c] = mxl; }
         } else {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            const Kv4Norm norm(sum, mx, mxl);
             const int t = row_of(a, c0 + c);
             uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs +
                            (long)(head * a.group + c0 + c - t * a.group) * a.out.hs + d;
-            *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+            *(uint2 *)op = make_uint2(pack_bf16(norm(o.x), norm(o.y)), pack_bf16(norm(o.z), norm(o.w)));
         }
     }
     __syncthreads();        // the stages are the next piece's
@@ -838,8 +888,8 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     }
 }
 
-// Joins the pieces of one column of a segment that was cut: weights
-// 2^(m_c - max m), in the order of the runs.  What it reads is on its way
+// Joins the pieces of one column of a segment that was cut: factors
+// 2^(m_c - max m), and for the sums those of their own maxima, in the order of the runs.  What it reads is on its way
 // together: each thread's first AHEAD pieces before the weights are known.
 // Two forms (kv4_attn_launch): WIDE for few columns, which may be cut into many
 // pieces; the other for many, of few pieces each.
@@ -848,7 +898,7 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
     constexpr int L = D / 4, P = (WIDE ? 256 : 128) / L, AHEAD = WIDE ? 8 : 1;
         // lanes over the dims, parts over the pieces
     extern __shared__ float kj_dyn[];                 // weights of the pieces, then [P][D] sums
-    __shared__ float total_s;
+    __shared__ float total_s, max_s, max_l_s;
     const int seq = blockIdx.z, head = blockIdx.y;
     Kv4Work wk = kv4_work(a, seq, cols_block, 1);
     const Kv4Seq sq = wk.sq;
@@ -863,31 +913,37 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
         const long i0 = runs == total ? b : div_long((b + 1) * runs - 1, total);
         const long i1 = runs == total ? e - 1 : div_long(e * runs - 1, total);
         if (i0 == i1) continue;                       // written by its only run
-        const int n = (int)(i1 - i0) + 1, stride = cols_block * (D + 2);
+        const int n = (int)(i1 - i0) + 1, stride = kv4::part_floats(cols_block, D);
         const float *const parts = a.part + (size_t)i0 * 2 * (size_t)stride;
         auto piece = [&](int i) { return parts + (size_t)(2 * i + (i == 0 ? 1 : 0)) * (size_t)stride; };
-        const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L, at = 2 * cols_block + cc * D + d;
+        const int d = (threadIdx.x % L) * 4, part = threadIdx.x / L, at = 3 * cols_block + cc * D + d;
         float4 y[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; u++)
             y[u] = part + u * P < n ? *(const float4 *)(piece(part + u * P) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
         if (threadIdx.x < 32) {
-            float mx = kv4::NEG_INF;
+            float mx = kv4::NEG_INF, mxl = kv4::NEG_INF;
 #pragma unroll 4
-            for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, piece(i)[cc]);
+            for (int i = threadIdx.x; i < n; i += 32) {
+                mx = fmaxf(mx, piece(i)[cc]);
+                mxl = fmaxf(mxl, piece(i)[2 * cols_block + cc]);
+            }
 #pragma unroll
-            for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            for (int off = 16; off; off >>= 1) {
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                mxl = fmaxf(mxl, __shfl_xor_sync(0xffffffffu, mxl, off));
+            }
             float sum = 0.f;
 #pragma unroll 4
             for (int i = threadIdx.x; i < n; i += 32) {
-                const float mi = piece(i)[cc], li = piece(i)[cols_block + cc];
-                const float k = mi == kv4::NEG_INF && li == 0.f ? 0.f : ex2(mi - mx);
-                kj_dyn[i] = k;
-                sum += li * k;
+                const float mi = piece(i)[cc], li = piece(i)[cols_block + cc], mli = piece(i)[2 * cols_block + cc];
+                const bool none = mli == kv4::NEG_INF && li == 0.f;
+                kj_dyn[i] = none ? 0.f : pow2((int)(mi - mx));
+                sum += none ? 0.f : li * pow2((int)(mli - mxl));
             }
 #pragma unroll
             for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            if (threadIdx.x == 0) total_s = sum;
+            if (threadIdx.x == 0) { total_s = sum; max_s = mx; max_l_s = mxl; }
         }
         __syncthreads();
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -903,10 +959,10 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
         if (part == 0) {
 #pragma unroll
             for (int i = 1; i < P; i++) add(*(const float4 *)(sums + i * D + d), 1.0f);
-            const float inv = total_s == 0.f ? 0.f : 1.0f / total_s;
+            const Kv4Norm norm(total_s, max_s, max_l_s);
             const int t = row_of(a, c);
             uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs + (long)(head * a.group + c - t * a.group) * a.out.hs + d;
-            *(uint2 *)op = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+            *(uint2 *)op = make_uint2(pack_bf16(norm(o.x), norm(o.y)), pack_bf16(norm(o.z), norm(o.w)));
         }
         __syncthreads();                              // the next column's weights and sums
     }
@@ -935,7 +991,7 @@ Kv4Plan kv4_plan(const Kv4View &v, size_t q_heads) {
     p.grid = (int)(most < p.slots ? most : p.slots);
     p.plan_bytes = ((size_t)v.nseq + 3) * sizeof(long);
     p.plan_bytes = (p.plan_bytes + 15) / 16 * 16;
-    p.bytes = p.whole ? 0 : p.plan_bytes + (size_t)p.grid * 2 * (8 * p.nt) * (v.dim + 2) * sizeof(float);
+    p.bytes = p.whole ? 0 : p.plan_bytes + (size_t)p.grid * 2 * kv4::part_floats(8 * p.nt, v.dim) * sizeof(float);
     return p;
 }
 

@@ -115,10 +115,12 @@ int apus_gcuda_kv4_read_dev(const ApusKv4Cache *cache, const ApusKv4Batch *batch
  * sel[r * sel_stride + j / pool] != 0 (0 beyond sel_stride), and always the
  * positions of its own last, incomplete pool.
  *
- * Scores, softmax statistics and sums are fp32; a weight is rounded to f16 as
- * it is and once more times its value's scale, for the tensor cores (2^-11
- * each; a power of two a position keeps both in f16's range, and what is below
- * 2^-30 of a row's largest term may add nothing).  Positions in a page whose id
+ * Scores, softmax statistics and sums are fp32, and the sum of the weights goes
+ * by the scores alone, however large or small the values are.  For the output a
+ * weight is rounded to f16 as it is and once more times its value's scale, for
+ * the tensor cores (2^-11 each; a power of two a position keeps both in f16's
+ * range, and a term, weight times value, below 2^-30 of a row's largest may add
+ * nothing).  Positions in a page whose id
  * is out of range count as unseen; a row that sees nothing gives zeros.  What
  * stands at unseen positions has no influence, NaN and infinities included; a
  * NaN or an infinity in a query row makes that row NaN, and a group of values
