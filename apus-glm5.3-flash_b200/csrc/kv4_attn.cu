@@ -393,8 +393,9 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     const CodeConst cc = code_const();
     // A unit's scales as the loop below wants them.  A position's value scales
     // are 2^E times numbers below 2, exact in f16 (those below 2^-24 of the
-    // largest become 0); E is -112 at least, so that 2^-E stays finite.  Whole
-    // warp; a lane takes four scales of each kind.
+    // largest become 0); E is kept to -126 .. 126, so that 2^-E is a normal number
+    // (a scale of 2^127 is then below 4, and a weight of 2^13 times that fits f16).
+    // Whole warp; a lane takes four scales of each kind.
     auto prepare = [&](const uint8_t *st) {
         static_assert(U * NG == 128, "four scales of keys and of values a lane");
         const uint2 k = *(const uint2 *)(st + C::KS + lane * 8), v = *(const uint2 *)(st + C::VS + lane * 8);
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
 #pragma unroll
         for (int u = 0; u < (NG == 2 ? 2 : 1); u++) {
             int e = (int)(__float_as_uint(top[u]) >> 23) - 127;    // a NaN's or an infinity's scales stay what they are
-            e = max(min(e, 120), -112);
+            e = max(min(e, 126), -126);
             inv[u] = __int_as_float((127 - e) << 23);
             const int r = NG == 2 ? 2 * lane + u : lane / (NG / 4);
             *(float *)(own + C::PW + r * 4) = (float)e;

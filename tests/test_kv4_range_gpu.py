@@ -72,3 +72,15 @@ def test_tiny_values_over_a_long_context(gcuda, dim, group, power):
     v = v.abs()
     got = run(gcuda, dim, 1, group, k, v, bf16(g, 1, group, dim).cuda())
     assert (got > 0).all()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 16), (256, 1)])
+@pytest.mark.parametrize("size", [8e37, 3e38])
+def test_largest_values_with_rising_scores(gcuda, dim, group, size):
+    """Values at the type's upper end whose weights rise by 7.9 powers of two after the first ones."""
+    for n in (100, 3000):
+        g = gen(n)
+        k, v = level(g, n, 1, dim, torch.full((n,), size))
+        k[20:] = torch.tensor(7.9 * math.log(2.0) * 8 / dim).to(torch.bfloat16)
+        got = run(gcuda, dim, 1, group, k, v, torch.ones(1, group, dim, dtype=torch.bfloat16).cuda())
+        assert got.isfinite().all()
