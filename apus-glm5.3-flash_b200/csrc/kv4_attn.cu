@@ -31,10 +31,11 @@
 //   * Scales are unpacked once a unit, not once a lane that needs them: fp32 for
 //     the keys; for the values f16 below 2, with a power of two a position that
 //     goes into the weight's exponent.  Two f16 roundings (2^-11 each) a weight.
-//   * So there are two running maxima: of z + E (2^E a position's power of two)
-//     for the output's weights, and of z alone for their sum, whose exponentials
-//     are computed a second time.  One weight for both, times 2^-E in the sum, lost
-//     a position whose values are zero or 2^127 below the others', or overflowed.
+//   * So there are two running maxima: ml of z for the sum of the weights, 2^(z - ml),
+//     and m of (z - ml) + E (2^E a position's power of two) for the output's, whose
+//     exponentials are computed a second time.  One weight for both, times 2^-E in the
+//     sum, lost a position whose values are zero or 2^127 below the others', or
+//     overflowed; and z + E without z - ml first rounds E away where scores are huge.
 // (E4M3 mma.sync looks four times as fast but is carried out as conversions and
 // f16 products: 50 conversions for 16 positions of dim 128, and no faster.)
 //
@@ -98,7 +99,7 @@ constexpr float NEG_INF = -__builtin_huge_valf();
 // A maximum is raised when a term passes it by more than 2^OVER (the output's weights
 // are f16) or 2^L_OVER (the sum is fp32 and has room for 2^67 such terms).
 constexpr float OVER = 13.0f, L_OVER = 60.0f;
-// A partial result: maximum, sum and the sum's maximum of each column, then its dims.
+// A partial result: m, sum and ml of each column, then its dims.
 constexpr int part_floats(int cols, int dim) { return cols * (dim + 3); }
 }  // namespace kv4
 
@@ -171,12 +172,11 @@ APUS_DEV float ex2(float x) {
 // rescale is not rounded.  (The difference of two infinities, NaN, counts as 0: it
 // arises where no position is seen, or in rows that are NaN already.)
 APUS_DEV float pow2(int e) { return __int_as_float(max(min(e, 127) + 127, 0) << 23); }
-// o / sum, brought from the output's maximum m to the sum's maximum ml: by two factors,
-// since m - ml goes from -140 to 187 and the result alone has to fit.
+// o 2^m / sum, by two factors: m goes from -140 to 187, and the result alone has to fit.
 struct Kv4Norm {
     float inv, a, b;
-    APUS_DEV Kv4Norm(float sum, float m, float ml) {
-        const int d = max(min((int)(m - ml), 250), -250);
+    APUS_DEV Kv4Norm(float sum, float m) {
+        const int d = max(min((int)m, 250), -250);
         inv = sum == 0.f ? 0.f : 1.0f / sum;
         a = pow2(d >> 1);
         b = pow2(d - (d >> 1));
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     uint32_t Q[C::QS ? 1 : NT][C::QS ? 1 : NG][4];
     float cinit[NT][NG][2], fac[NT][2];
     int lim[NT][2];
-    // columns 2 q4, 2 q4 + 1: output and its maximum (of z + E), the sum of this lane's
-    // weights and its maximum (of z)
+    // columns 2 q4, 2 q4 + 1: output and its maximum, the sum of this lane's weights and
+    // its maximum
     float O[NT][D / 16][4], m[NT][2], l[NT][2], ml[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -479,13 +479,22 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                 f32_unpair(mul_f32x2(z2[nt][1], f), z[nt][2], z[nt][3]);
             }
         }
-        // ---- running maximum of z + E, so of what a position adds to the output:
-        // its weight times 2^E, and times a scale below 2, then fits f16 with the
-        // largest at 2^5 to 2^13 whatever the scales' range (what is below 2^-30 of
-        // the largest may add nothing).  That of z, for the sum.
+        // ---- running maxima: ml of z, m of y + E, y = z - ml, so of what a position adds
+        // to the output: its weight times 2^E, and times a scale below 2, then fits f16
+        // with the largest at 2^5 to 2^13 whatever the scales' range (what is below 2^-30
+        // of the largest may add nothing).
         uint32_t hide = 0;             // bit nt * 4 + i (MASKED)
         bool over = false;
-        float ze[NT][4], high[NT][2], high_l[NT][2];
+        float y[NT][4], ye[NT][4];     // y and y + E - m
+        auto relate = [&](int nt) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint64_t d = add_f32x2(f32_pair(z[nt][2 * h], z[nt][2 * h + 1]), f32_pair(-ml[nt][0], -ml[nt][1]));
+                f32_unpair(d, y[nt][2 * h], y[nt][2 * h + 1]);
+                f32_unpair(add_f32x2(add_f32x2(d, f32_pair(pw[h], pw[h])), f32_pair(-m[nt][0], -m[nt][1])), ye[nt][2 * h],
+                           ye[nt][2 * h + 1]);
+            }
+        };
         uint32_t name[2] = {0, 0};
         if (SEL) { name[0] = names[pg]; name[1] = names[pg + 8]; }
 #pragma unroll
@@ -498,40 +507,38 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                     if (!see) { z[nt][i] = NEG_INF; hide |= 1u << (nt * 4 + i); }
                 }
             }
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-                f32_unpair(add_f32x2(f32_pair(z[nt][2 * h], z[nt][2 * h + 1]), f32_pair(pw[h], pw[h])), ze[nt][2 * h],
-                           ze[nt][2 * h + 1]);
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                high[nt][u] = fmaxf(ze[nt][u], ze[nt][u + 2]);
-                high_l[nt][u] = fmaxf(z[nt][u], z[nt][u + 2]);
-                over |= high[nt][u] > m[nt][u] + kv4::OVER || high_l[nt][u] > ml[nt][u] + kv4::L_OVER;
-            }
+            relate(nt);
+            over |= fmaxf(fmaxf(fmaxf(y[nt][0], y[nt][1]), y[nt][2]), y[nt][3]) > kv4::L_OVER;
+            over |= fmaxf(fmaxf(fmaxf(ye[nt][0], ye[nt][1]), ye[nt][2]), ye[nt][3]) > kv4::OVER;
         }
         if (__any_sync(0xffffffffu, over)) {
+            auto highest = [&](float x, float x2) {
+                x = fmaxf(x, x2);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+                return x;
+            };
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {                      // each column by its own scores alone
+                    const float x = highest(z[nt][u], z[nt][u + 2]), up = floorf(x) - ml[nt][u];
+                    if (!(x - ml[nt][u] > kv4::L_OVER)) continue;
+                    l[nt][u] *= pow2((int)-up);
+                    ml[nt][u] = floorf(x);
+                    m[nt][u] -= up;                                // (of -inf: stays that)
+                }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    float x = high[nt][u], xl = high_l[nt][u];
-#pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) {
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                        xl = fmaxf(xl, __shfl_xor_sync(0xffffffffu, xl, off));
-                    }
-                    if (xl > ml[nt][u] + kv4::L_OVER) {            // each column by its own scores alone
-                        xl = floorf(xl);
-                        l[nt][u] *= pow2((int)(ml[nt][u] - xl));
-                        ml[nt][u] = xl;
-                    }
-                    if (!(x > m[nt][u] + kv4::OVER)) continue;
-                    x = floorf(x) - 5.0f;
-                    const float down = pow2((int)(m[nt][u] - x));
-                    m[nt][u] = x;
+                    const float x = highest(z[nt][u] - ml[nt][u] + pw[0], z[nt][u + 2] - ml[nt][u] + pw[1]), to = floorf(x) - 5.0f;
+                    if (!(x - m[nt][u] > kv4::OVER)) continue;
+                    const float down = pow2((int)(m[nt][u] - to));
+                    m[nt][u] = to;
 #pragma unroll
                     for (int i = 0; i < D / 16; i++) { O[nt][i][u] *= down; O[nt][i][u + 2] *= down; }
                 }
+                relate(nt);
+            }
         }
         // ---- weights (times 2^E), brought to the order of the output's operand:
         // column g, positions 0, 1 and 2, 3 of the lane
@@ -540,16 +547,13 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         for (int nt = 0; nt < NT; nt++) {
             float p[4];
             uint64_t sum = f32_pair(l[nt][0], l[nt][1]);
-            const uint64_t down = f32_pair(-m[nt][0], -m[nt][1]), down_l = f32_pair(-ml[nt][0], -ml[nt][1]);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 float w[2];
-                f32_unpair(add_f32x2(f32_pair(ze[nt][2 * h], ze[nt][2 * h + 1]), down), p[2 * h], p[2 * h + 1]);
-                f32_unpair(add_f32x2(f32_pair(z[nt][2 * h], z[nt][2 * h + 1]), down_l), w[0], w[1]);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    p[2 * h + u] = ex2(p[2 * h + u]);
-                    w[u] = ex2(w[u]);
+                    p[2 * h + u] = ex2(ye[nt][2 * h + u]);
+                    w[u] = ex2(y[nt][2 * h + u]);
                     // a hidden position adds nothing to the sum, and its weight is -0: the sign
                     // marks it below, where a NaN scale must not reach the product
                     if (MASKED && (hide >> (nt * 4 + 2 * h + u) & 1)) { p[2 * h + u] = -0.0f; w[u] = 0.f; }
@@ -857,27 +861,26 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     float *part = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * (size_t)kv4::part_floats(COLS, D);
     for (int i = threadIdx.x; i < (cend - c0) * (D / 4); i += kv4::THREADS) {
         const int c = i / (D / 4), d = (i % (D / 4)) * 4;
-        float mx = NEG_INF, mxl = NEG_INF;
+        float mx = NEG_INF, mxl = NEG_INF;         // ml of all, m relative to that
 #pragma unroll
-        for (int w = 0; w < kv4::WARPS; w++) {
-            mx = fmaxf(mx, join_m[w][c]);
-            mxl = fmaxf(mxl, join_ml[w][c]);
-        }
+        for (int w = 0; w < kv4::WARPS; w++) mxl = fmaxf(mxl, join_ml[w][c]);
+#pragma unroll
+        for (int w = 0; w < kv4::WARPS; w++) mx = fmaxf(mx, join_m[w][c] + (join_ml[w][c] - mxl));
         float sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kv4::WARPS; w++) {
             if (join_ml[w][c] == NEG_INF && join_l[w][c] == 0.f) continue;
-            const float k = pow2((int)(join_m[w][c] - mx));
+            const float up = join_ml[w][c] - mxl, k = pow2((int)(join_m[w][c] + up - mx));
             const float4 x = *(const float4 *)(jo + (w * COLS + c) * JD + d);
-            sum += join_l[w][c] * pow2((int)(join_ml[w][c] - mxl));
+            sum += join_l[w][c] * pow2((int)up);
             o.x += x.x * k; o.y += x.y * k; o.z += x.z * k; o.w += x.w * k;
         }
         if (!last) {
             *(float4 *)(part + 3 * COLS + c * D + d) = o;
             if (d == 0) { part[c] = mx; part[COLS + c] = sum; part[2 * COLS + c] = mxl; }
         } else {
-            const Kv4Norm norm(sum, mx, mxl);
+            const Kv4Norm norm(sum, mx);
             const int t = row_of(a, c0 + c);
             uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs +
                            (long)(head * a.group + c0 + c - t * a.group) * a.out.hs + d;
@@ -889,8 +892,9 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
     }
 }
 
-// Joins the pieces of one column of a segment that was cut: factors
-// 2^(m_c - max m), and for the sums those of their own maxima, in the order of the runs.  What it reads is on its way
+// Joins the pieces of one column of a segment that was cut: the maxima ml, then the m
+// relative to the largest of them, then the sums with factors from these, in the order
+// of the runs.  What it reads is on its way
 // together: each thread's first AHEAD pieces before the weights are known.
 // Two forms (kv4_attn_launch): WIDE for few columns, which may be cut into many
 // pieces; the other for many, of few pieces each.
@@ -898,8 +902,8 @@ template <int D, bool WIDE>
 __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(const Kv4AttnArgs a, int cols_block) {
     constexpr int L = D / 4, P = (WIDE ? 256 : 128) / L, AHEAD = WIDE ? 8 : 1;
         // lanes over the dims, parts over the pieces
-    extern __shared__ float kj_dyn[];                 // weights of the pieces, then [P][D] sums
-    __shared__ float total_s, max_s, max_l_s;
+    extern __shared__ float kj_dyn[];                 // m (then weights), sums and ml of the pieces, then [P][D] sums
+    __shared__ float total_s, max_s;
     const int seq = blockIdx.z, head = blockIdx.y;
     Kv4Work wk = kv4_work(a, seq, cols_block, 1);
     const Kv4Seq sq = wk.sq;
@@ -924,27 +928,32 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
             y[u] = part + u * P < n ? *(const float4 *)(piece(part + u * P) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
         if (threadIdx.x < 32) {
             float mx = kv4::NEG_INF, mxl = kv4::NEG_INF;
+            // (a lane finds its own pieces' in shared memory again)
+            float *const km = kj_dyn, *const kl = kj_dyn + KJ_RUNS, *const kml = kj_dyn + 2 * KJ_RUNS;
 #pragma unroll 4
             for (int i = threadIdx.x; i < n; i += 32) {
-                mx = fmaxf(mx, piece(i)[cc]);
-                mxl = fmaxf(mxl, piece(i)[2 * cols_block + cc]);
+                km[i] = piece(i)[cc];
+                kl[i] = piece(i)[cols_block + cc];
+                const float mli = kml[i] = piece(i)[2 * cols_block + cc];
+                mxl = fmaxf(mxl, mli);
             }
 #pragma unroll
-            for (int off = 16; off; off >>= 1) {
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                mxl = fmaxf(mxl, __shfl_xor_sync(0xffffffffu, mxl, off));
-            }
+            for (int off = 16; off; off >>= 1) mxl = fmaxf(mxl, __shfl_xor_sync(0xffffffffu, mxl, off));
+#pragma unroll 4
+            for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, km[i] + (kml[i] - mxl));
+#pragma unroll
+            for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             float sum = 0.f;
 #pragma unroll 4
             for (int i = threadIdx.x; i < n; i += 32) {
-                const float mi = piece(i)[cc], li = piece(i)[cols_block + cc], mli = piece(i)[2 * cols_block + cc];
+                const float mi = km[i], li = kl[i], mli = kml[i];
                 const bool none = mli == kv4::NEG_INF && li == 0.f;
-                kj_dyn[i] = none ? 0.f : pow2((int)(mi - mx));
+                kj_dyn[i] = none ? 0.f : pow2((int)(mi + (mli - mxl) - mx));
                 sum += none ? 0.f : li * pow2((int)(mli - mxl));
             }
 #pragma unroll
             for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            if (threadIdx.x == 0) { total_s = sum; max_s = mx; max_l_s = mxl; }
+            if (threadIdx.x == 0) { total_s = sum; max_s = mx; }
         }
         __syncthreads();
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -954,13 +963,13 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
             if (part + u * P < n) add(y[u], kj_dyn[part + u * P]);
 #pragma unroll 4
         for (int i = part + AHEAD * P; i < n; i += P) add(*(const float4 *)(piece(i) + at), kj_dyn[i]);
-        float *const sums = kj_dyn + KJ_RUNS;
+        float *const sums = kj_dyn + 3 * KJ_RUNS;
         *(float4 *)(sums + part * D + d) = o;
         __syncthreads();
         if (part == 0) {
 #pragma unroll
             for (int i = 1; i < P; i++) add(*(const float4 *)(sums + i * D + d), 1.0f);
-            const Kv4Norm norm(total_s, max_s, max_l_s);
+            const Kv4Norm norm(total_s, max_s);
             const int t = row_of(a, c);
             uint16_t *op = a.out.p + (long)(sq.row0 + t) * a.out.rs + (long)(head * a.group + c - t * a.group) * a.out.hs + d;
             *(uint2 *)op = make_uint2(pack_bf16(norm(o.x), norm(o.y)), pack_bf16(norm(o.z), norm(o.w)));
@@ -1033,7 +1042,7 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)bx, a.v.heads, a.v.nseq);
     cfg.blockDim = dim3(wide ? 256 : 128);
-    cfg.dynamicSmemBytes = (KJ_RUNS + (wide ? 256 : 128) * 4) * 4;
+    cfg.dynamicSmemBytes = (3 * KJ_RUNS + (wide ? 256 : 128) * 4) * 4;
     cfg.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -84,3 +84,46 @@ def test_largest_values_with_rising_scores(gcuda, dim, group, size):
         k[20:] = torch.tensor(7.9 * math.log(2.0) * 8 / dim).to(torch.bfloat16)
         got = run(gcuda, dim, 1, group, k, v, torch.ones(1, group, dim, dtype=torch.bfloat16).cuda())
         assert got.isfinite().all()
+
+
+def test_huge_scores(gcuda):
+    """Scores of 2^27 and more, where neighbouring fp32 numbers are 8 to 16 apart: the later positions' lie one such
+    step above the first ones'.  Whatever the rounding of the scores, an output lies between the values."""
+    dim, lens = 64, [40] * 48
+    k = torch.zeros(sum(lens), 1, dim)
+    v = torch.ones(sum(lens), 1, dim)
+    v[:, :, 1] = -1.0
+    for i in range(len(lens)):
+        k[40 * i:40 * i + 40, 0, :32] = 2.0 ** 22 * (1 + i / 64)          # 2^27 (1 + i / 64) with q of ones
+        k[40 * i + 20:40 * i + 40, 0, 32:] = (4 + i % 8) / 32.0           # 4 to 11 more
+    c = Case(gcuda, dim, 1, lens, [1] * len(lens), seed=3)
+    c.write_all(k.to(torch.bfloat16), v.to(torch.bfloat16))
+    q = torch.ones(len(lens), 2, dim, dtype=torch.bfloat16).cuda()
+    got = c.attn(q, 1.0)
+    torch.cuda.synchronize()
+    want = torch.ones(len(lens), 2, dim)
+    want[:, :, 1] = -1.0
+    # every value is the same: weights of 2^-11 and a BF16 rounding
+    assert ((got.float().cpu() - want).abs() <= R.U + 2 * R.H).all()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 2), (128, 16), (256, 1)])
+@pytest.mark.parametrize("power", [6, 12, 16, 20, 24, 30])
+def test_large_scores(gcuda, dim, group, power):
+    """Scores of about 2^power that differ from position to position: whatever their rounding, equal values come out
+    as they are (each weight off by two f16 roundings, the sums by fp32's, the result by a BF16 rounding)."""
+    for n in (90, 3000):
+        g = gen(power)
+        k = bf16(g, n, 1, dim)
+        k[:, :, 0] = 7.0
+        v = torch.full((n, 1, dim), 3.0e-2)
+        v[:, :, 1::2] = -7.0
+        c = Case(gcuda, dim, 1, [n], [1], seed=power)
+        c.write_all(k, v.to(torch.bfloat16))
+        q = bf16(g, 1, group, dim)
+        q[:, :, 0] = 2.0 ** power / 7.0
+        held = c.v[0, 0].float()
+        for sel in (None, torch.ones(1, n, dtype=torch.uint8).cuda()):
+            got = c.attn(q.cuda(), 1.0, sel, 0 if sel is None else 1)
+            torch.cuda.synchronize()
+            assert ((got.float().cpu() - held).abs() <= held.abs() * (R.U + 2 * R.H + 2.0 ** -18)).all()
