@@ -117,10 +117,16 @@ int apus_gcuda_kv4_read_dev(const ApusKv4Cache *cache, const ApusKv4Batch *batch
  *
  * Scores, softmax statistics and sums are fp32, and the sum of the weights goes
  * by the scores alone, however large or small the values are.  For the output a
- * weight is rounded to f16 as it is and once more times its value's scale, for
- * the tensor cores (2^-11 each; a power of two a position keeps both in f16's
- * range, and a term, weight times value, below 2^-30 of a row's largest may add
- * nothing).  Positions in a page whose id
+ * weight w is rounded to f16 as it is and once more times its value's scale s,
+ * for the tensor cores, in units of a power of two that keep the row's largest
+ * w s in f16's range; scales are f16 too, relative to their position's largest
+ * (exact from 2^-17 of that on).  So a term w s c (c the code) is off by 2^-10
+ * of itself, plus 21 * 2^-30 of the row's largest w s in any group, plus
+ * 7 * 2^-25 of the largest w s of its position: groups of dims 2^14 and more
+ * below their neighbours lose bits, and at 2^25 below they count as zeros.
+ * Query elements are exact down to 2^-24 of their row's largest and held to
+ * 2^-35 of it below; a row whose largest magnitude times scale is 2^117 or more
+ * may be NaN.  Positions in a page whose id
  * is out of range count as unseen; a row that sees nothing gives zeros.  What
  * stands at unseen positions has no influence, NaN and infinities included; a
  * NaN or an infinity in a query row makes that row NaN, and a group of values
@@ -155,7 +161,10 @@ typedef struct {
  * cores.  A row that sees no key gives zeros; keys and values that a row does
  * not see have no influence on it, NaN and infinities included; rows behind
  * cu_q[nseq] are left as they are.  Out of bounds, a sequence's range counts
- * as no queries or no keys. */
+ * as no queries or no keys.  Scores are bounded by fp32 before the scale is
+ * applied, and so are the weighted sums before they are divided, in which a
+ * weight counts up to 2^8: with values of 2^120 / keys and more (10^32 at 10^4
+ * keys) they may overflow, and the row then holds infinities or NaN. */
 int apus_gcuda_prompt_attn_dev(const ApusPromptBatch *batch, const ApusHeadRows *q, const ApusHeadRows *k,
                                const ApusHeadRows *v, const ApusHeadRows *out, size_t dim, float scale, void *stream);
 

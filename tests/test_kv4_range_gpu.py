@@ -127,3 +127,22 @@ def test_large_scores(gcuda, dim, group, power):
             got = c.attn(q.cuda(), 1.0, sel, 0 if sel is None else 1)
             torch.cuda.synchronize()
             assert ((got.float().cpu() - held).abs() <= held.abs() * (R.U + 2 * R.H + 2.0 ** -18)).all()
+
+
+def test_query_beyond_the_scores(gcuda):
+    """A query whose factor passes fp32 makes its rows NaN, whatever the keys' signs; the others are as before."""
+    g = gen(4)
+    c = Case(gcuda, 128, 1, [70, 700, 20], [2, 1, 1], seed=4)
+    k, v = bf16(g, 790, 1, 128).abs(), bf16(g, 790, 1, 128)
+    c.write_all(k, v)
+    q = bf16(g, 4, 2, 128).cuda()
+    want = c.attn(q, 0.1)
+    for sign in (1.0, -1.0):
+        big = q.clone()
+        big[1, 0] = sign * 3e38
+        big[2, 1] = big[3, 0] = sign * 3e38
+        got = c.attn(big, 0.1)
+        torch.cuda.synchronize()
+        assert got[1, 0].isnan().all() and got[2, 1].isnan().all() and got[3, 0].isnan().all()
+        got[1, 0], got[2, 1], got[3, 0] = want[1, 0], want[2, 1], want[3, 0]
+        assert torch.equal(got, want)
