@@ -54,7 +54,6 @@ struct Kv4Place { int page, off; bool in; };
 APUS_DEV Kv4Place kv4_place(const Kv4View &v, int row, bool report) {
     const int s = seq_of_row(v.cu, v.nseq, row);
     const Kv4Seq q = kv4_seq(v.cu[s], v.cu[s + 1], v.len[s], v.rows, v.max_rows, v.max_len);
-    if (q.bad && report) atomicExch(&g_kv4_err, (int)ATTN_ERR_SEQ);
     Kv4Place pl{-1, 0, row >= q.row0 && row < q.row0 + q.n};
     const int pos = q.len - q.n + (row - q.row0);
     if (!pl.in || pos < 0) return pl;
@@ -66,6 +65,16 @@ APUS_DEV Kv4Place kv4_place(const Kv4View &v, int row, bool report) {
         atomicExch(&g_kv4_err, (int)ATTN_ERR_PAGE);
     }
     return pl;
+}
+
+// Reports every sequence out of bounds, those that no row leads to among them (the
+// grid's first row of blocks, a thread a sequence while there are enough).
+APUS_DEV void kv4_report(const Kv4View &v) {
+    if (blockIdx.y || blockIdx.x >= 256) return;      // (at most 65535 sequences)
+#pragma unroll 1
+    for (int s = blockIdx.x * 256 + threadIdx.x; s < v.nseq; s += min(gridDim.x, 256) * 256)
+        if (kv4_seq(v.cu[s], v.cu[s + 1], v.len[s], v.rows, v.max_rows, v.max_len).bad)
+            atomicExch(&g_kv4_err, (int)ATTN_ERR_SEQ);
 }
 
 // Thread -> eight dims (c) of a row; items blockIdx.y * IT .. + IT - 1 of the
@@ -94,6 +103,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(Kv4View v, RowsView k, RowsV
     }
     Kv4Place pl{-1, 0, false};
     if (on) pl = kv4_place(v, (int)me.row, c == 0);
+    kv4_report(v);
     const int j = c >> 2, q4 = c & 3;            // group of 32 dims, quarter of it
 #pragma unroll
     for (int i = 0; i < IT; i++) {
@@ -155,6 +165,7 @@ __global__ void __launch_bounds__(256) k_kv4_append(Kv4View v, RowsView k, RowsV
 template <int D, int IT>
 __global__ void __launch_bounds__(256) k_kv4_read(Kv4View v, RowsView k, RowsView x) {
     const Kv4Part<D> me;
+    kv4_report(v);
     if (me.row >= v.rows) return;
     const int c = me.c, items = 2 * v.heads, it0 = blockIdx.y * IT;
     const Kv4Place pl = kv4_place(v, (int)me.row, c == 0);

@@ -78,7 +78,10 @@ typedef struct {
  * Position p is in page page_table[s * table_stride + p / 64].  max_rows and
  * max_len bound the rows and the length of any sequence (max_len <=
  * 64 * table_stride).  A sequence may have no rows or no positions (padding of
- * a batch).  Out of bounds, a length counts as 0 and a row range as no rows. */
+ * a batch).  Out of bounds, a length counts as 0 and a row range as no rows.
+ * cu_rows ascends: where it does not, a range is out of bounds and reported, and
+ * append and read, which look a row's sequence up, may also leave out rows of
+ * other sequences. */
 typedef struct {
     const int32_t *cu_rows;      /* [nseq + 1] */
     const int32_t *kv_len;       /* [nseq], this call's rows included */
