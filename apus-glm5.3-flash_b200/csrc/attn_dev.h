@@ -7,7 +7,8 @@
 
 static_assert(KV4_PAGE == APUS_KV4_PAGE && KV4_GROUP == APUS_KV4_GROUP, "public and internal layout");
 
-enum { ATTN_ERR_PAGE = 41, ATTN_ERR_SEQ = 42, ATTN_ERR_WAIT = 43 };   // 43..: a bounded wait gave up
+// The worse, the larger: an error word is raised with atomicMax.  43: a bounded wait gave up.
+enum { ATTN_ERR_PAGE = 41, ATTN_ERR_SEQ = 42, ATTN_ERR_WAIT = 43 };
 
 // Device views of the public structs (sizes checked to fit ints).
 struct Kv4View {

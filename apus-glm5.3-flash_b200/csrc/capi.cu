@@ -1,6 +1,7 @@
 // capi.cu — the C ABI of include/apus_gcuda.h: error plumbing, HBM
 // residency registry, host-pointer drop-ins and device-pointer twins of the
 // linear leaf.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -249,10 +250,9 @@ void apus_gcuda_clear_error(void) { g_err[0] = 0; }
 int apus_gcuda_kernel_error(void) {
     cudaDeviceSynchronize();
     const int a = kernel_error_read_and_clear(), b = ep_error_read_and_clear(), c = tc_error_read_and_clear();
-    if (a || b || c) return a ? a : (b ? b : c);
-    const int k = kv4_cache_error_read_and_clear(), l = kv4_attn_error_read_and_clear(),
-              p = prompt_attn_error_read_and_clear();
-    return k ? k : (l ? l : p);
+    const int attn = std::max({kv4_cache_error_read_and_clear(), kv4_attn_error_read_and_clear(),
+                               prompt_attn_error_read_and_clear()});
+    return a ? a : (b ? b : (c ? c : attn));
 }
 
 int apus_gcuda_register_region(const void *ptr, size_t len) {

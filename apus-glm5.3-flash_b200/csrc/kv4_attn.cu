@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         if (s < a.v.nseq) {
             if (!again) {
                 const Kv4Work k = kv4_work(a, s, COLS, 1);
-                if (k.sq.bad && blockIdx.x == 0) atomicExch(&g_kv4a_err, (int)ATTN_ERR_SEQ);
+                if (k.sq.bad && blockIdx.x == 0) atomicMax(&g_kv4a_err, (int)ATTN_ERR_SEQ);
                 per_unit = a.v.heads * k.ncb;
                 pages = (int)k.units;
             }
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                         if (i + lane < mine) {
                             const int page = table[(p0 + (u + lane * kv4::WARPS) * U) / KV4_PAGE];
                             if (kv4_page_ok(page, a.v.num_pages)) my_page = page;
-                            else atomicExch(&g_kv4a_err, (int)ATTN_ERR_PAGE);
+                            else atomicMax(&g_kv4a_err, (int)ATTN_ERR_PAGE);
                         }
                     }
                     const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                             off[e] = j & (KV4_PAGE - 1);
                             if (kv4_page_ok(page, a.v.num_pages)) src[e] = a.v.pages + kv4_block_at(page, head, a.v.heads, D);
                             else {
-                                atomicExch(&g_kv4a_err, (int)ATTN_ERR_PAGE);
+                                atomicMax(&g_kv4a_err, (int)ATTN_ERR_PAGE);
                                 list[u0 + r] &= 0xffffu;   // no row sees it
                             }
                         }

@@ -39,7 +39,9 @@ const char *apus_gcuda_last_error(void);
 void apus_gcuda_clear_error(void);
 /* Device-side error word of the pipelined kernels (0 = none; nonzero = a
  * bounded wait gave up: 1 producer, 2 consumer; 41-43: the operators of
- * apus_attn_gcuda.h), read and cleared.  Synchronises the device. */
+ * apus_attn_gcuda.h), read and cleared.  Where several were recorded since the
+ * last call, the one returned is a wait's before any other and of 41-43 the
+ * largest; all are cleared.  Synchronises the device. */
 int apus_gcuda_kernel_error(void);
 
 /* Persistent HBM residency for a model-owned host weight region: the bytes
