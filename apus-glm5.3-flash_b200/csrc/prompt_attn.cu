@@ -49,6 +49,8 @@
 // (and all rows behind the sequence) are set to 0 in shared memory before the
 // product reads them; the first key with a NaN, a +inf and a -inf is kept for each
 // dim, and the rows that see it get it added at the end.
+#include <atomic>
+
 #include "attn_dev.h"
 #include "common.cuh"
 #include "pipe.cuh"
@@ -727,7 +729,9 @@ using namespace apus;
 // 3-D BF16 tensor map of rows of heads (dims, heads, rows): boxes of 64 dims of
 // one head of 128 rows in the 128-byte swizzle; zeros past the last row.
 static int pa_map(CUtensorMap *m, const ApusHeadRows *r, size_t dim) {
-    static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+    // looked up again after a failure; first calls of several threads may each look it up
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> encoder{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 enc = encoder.load(std::memory_order_acquire);
     if (!enc) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -737,6 +741,7 @@ static int pa_map(CUtensorMap *m, const ApusHeadRows *r, size_t dim) {
             return -1;
         }
         enc = (PFN_cuTensorMapEncodeTiled_v12000)p;
+        encoder.store(enc, std::memory_order_release);
     }
     // the stride of an axis of one is not looked at, but has to be a valid one
     const cuuint64_t dims[3] = {dim, r->heads, r->rows};
