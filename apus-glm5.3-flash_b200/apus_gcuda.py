@@ -311,6 +311,9 @@ class Kv4Batch:
         n = kv_len.shape[0]
         if cu_rows.shape[0] != n + 1 or page_table.shape[0] != n:
             raise GcudaError(f"kv4 batch: {n} sequences, {cu_rows.shape[0]} row starts, {page_table.shape[0]} page lists")
+        # (a view's rows may be farther apart than it is wide: the library goes by their distance)
+        if not 0 <= max_len <= KV4_PAGE * page_table.shape[1]:
+            raise GcudaError(f"kv4 batch: {max_len} positions in a table of {page_table.shape[1]} pages")
         self.tensors, self.index = (cu_rows, kv_len, page_table), kv_len.get_device()
         if cu_rows.get_device() != self.index or page_table.get_device() != self.index:
             raise GcudaError(f"kv4 batch: tensors on {cu_rows.device}, {kv_len.device} and {page_table.device}")
