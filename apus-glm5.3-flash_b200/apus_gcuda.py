@@ -199,6 +199,9 @@ apus_gspec_step = _fn("apus_gspec_step", _i, _vp, _vp, _i)
 
 
 # ---- batched attention and the 4-bit cache (include/apus_attn_gcuda.h) ------
+# The calls run on torch's current stream, or on `stream`, a torch.cuda.Stream:
+# the caller orders it behind whatever wrote the inputs, and may drop its tensors
+# at once (they are recorded on it, so an ExternalStream has to outlive them).
 KV4_PAGE, KV4_GROUP = 64, 32
 
 
@@ -267,6 +270,16 @@ def _raw_stream(index, stream):
         return stream.cuda_stream
     import torch
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _record(stream, *tensors):
+    """Tells torch's allocator that a stream given by the caller uses the
+    tensors: freed early, their memory goes to nobody else before it is
+    through with them.  (On the current stream that is so without it.)"""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
 
 
 def _ints(what, t, dim):
@@ -351,6 +364,7 @@ def kv4_append(cache, batch, k, v, stream=None):
     _kv4_call("kv4_append", cache, batch, k, v)
     check(apus_gcuda_kv4_append_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"),
                                     _raw_stream(cache.index, stream)), "kv4_append")
+    _record(stream, cache.pages, *batch.tensors, k, v)
 
 
 def kv4_read(cache, batch, k, v, stream=None):
@@ -358,6 +372,7 @@ def kv4_read(cache, batch, k, v, stream=None):
     _kv4_call("kv4_read", cache, batch, k, v)
     check(apus_gcuda_kv4_read_dev(cache.ref, batch.ref, head_rows(k, "k"), head_rows(v, "v"),
                                   _raw_stream(cache.index, stream)), "kv4_read")
+    _record(stream, cache.pages, *batch.tensors, k, v)
 
 
 def kv4_attn_workspace(cache, batch, q_heads):
@@ -385,6 +400,7 @@ def kv4_attn(cache, batch, q, out, scale, workspace=None, sel=None, pool=0, stre
                                   None if workspace is None else workspace.data_ptr(),
                                   0 if workspace is None else workspace.numel() * workspace.element_size(),
                                   _raw_stream(cache.index, stream)), "kv4_attn")
+    _record(stream, cache.pages, *batch.tensors, q, out, workspace, sel)
 
 
 def prompt_attn(batch, q, k, v, out, scale, stream=None):
@@ -396,6 +412,7 @@ def prompt_attn(batch, q, k, v, out, scale, stream=None):
     _on("prompt_attn", batch.index, q, k, v, out)
     check(apus_gcuda_prompt_attn_dev(batch.ref, head_rows(q, "q"), head_rows(k, "k"), head_rows(v, "v"),
                                      head_rows(out, "out"), dim, scale, _raw_stream(batch.index, stream)), "prompt_attn")
+    _record(stream, *batch.tensors, q, k, v, out)
 
 
 EP_HANDLE_BYTES = 64   # sizeof(cudaIpcMemHandle_t)
