@@ -623,7 +623,15 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                         }
                     }
                 }
-                const float mz = m == -INFINITY ? 0.f : m * a.zscale;
+                float mz = m == -INFINITY ? 0.f : m * a.zscale;
+                // a product that is rounded to 2^-7 and more: the difference first, which is
+                // exact for neighbours (from 2^31 on, the rounding alone reached 2^127)
+                if (__any_sync(0xffffffffu, fabsf(mz) > 65536.0f)) {
+                    const uint64_t down = f32_pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+#pragma unroll
+                    for (int c = 0; c < 128; c += 2) f32_unpair(add_f32x2(f32_pair(v[c], v[c + 1]), down), v[c], v[c + 1]);
+                    mz = 0.f;
+                }
                 // two scores an instruction (packed fp32): the loop is a quarter shorter (dim 64
                 // 386 -> 357 us, seven ragged prompts 66 -> 63 us)
                 const uint64_t scale2 = f32_pair(a.zscale, a.zscale), mz2 = f32_pair(-mz, -mz);
