@@ -34,6 +34,23 @@ int kv4_check(const char *what, const ApusKv4Cache *c, const ApusKv4Batch *b, si
 static inline RowsView rows_view(const ApusHeadRows *r) {
     return RowsView{r->p, (long)r->row_stride, (long)r->head_stride};
 }
+// Launches a kernel and goes by what this launch returns: cudaGetLastError would also
+// give an error that an earlier call of the library left (a refused allocation, say).
+template <class... P, class... A>
+int attn_launch(const char *what, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, bool dependent,
+                const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = dependent ? 1 : 0;       // starts while the kernel before drains, and waits for it
+    return gcuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
 // the device error words
 int kv4_cache_error_read_and_clear(void);
 int kv4_attn_error_read_and_clear(void);

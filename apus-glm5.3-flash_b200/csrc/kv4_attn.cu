@@ -1030,8 +1030,7 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     using C = kv4::Cfg<D>;
     const int smem = C::SMEM + (SEL ? (kv4::LIST + 16) * 4 : 0);
     if (gcuda_smem_limit_once((const void *)k_kv4_attn<D, NT, SEL>, smem)) return -1;
-    k_kv4_attn<D, NT, SEL><<<grid, kv4::THREADS, smem, st>>>(a);
-    if (gcuda_check(cudaGetLastError(), "kv4_attn launch")) return -1;
+    if (attn_launch("kv4_attn launch", k_kv4_attn<D, NT, SEL>, dim3((unsigned)grid), kv4::THREADS, smem, st, false, a)) return -1;
     if (a.whole) return 0;
     // the joining kernel starts while the first drains, and waits for it: a block a
     // column, up to 64 (max_rows may be far above the rows that there are).  The wide
@@ -1039,18 +1038,9 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     // 47 with the other; 48 sequences, 384 segments: 69 us, 79 with the wide form).
     const long bx = std::min((long)a.group * a.v.max_rows, 64l);
     const bool wide = bx * a.v.heads * a.v.nseq <= 2 * 148;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)bx, a.v.heads, a.v.nseq);
-    cfg.blockDim = dim3(wide ? 256 : 128);
-    cfg.dynamicSmemBytes = (3 * KJ_RUNS + (wide ? 256 : 128) * 4) * 4;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return gcuda_check(cudaLaunchKernelEx(&cfg, wide ? k_kv4_join<D, true> : k_kv4_join<D, false>, a, 8 * NT),
-                       "kv4_attn join launch");
+    return attn_launch("kv4_attn join launch", wide ? k_kv4_join<D, true> : k_kv4_join<D, false>,
+                       dim3((unsigned)bx, a.v.heads, a.v.nseq), wide ? 256 : 128, (3 * KJ_RUNS + (wide ? 256 : 128) * 4) * 4, st,
+                       true, a, 8 * NT);
 }
 template <int D, int NT> int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     return a.sel ? kv4_attn_launch<D, NT, true>(a, grid, st) : kv4_attn_launch<D, NT, false>(a, grid, st);

@@ -226,9 +226,8 @@ static int kv4_rows_launch(const char *what, const Kv4View &view, const ApusHead
                            void *stream) {
     const long bx = ((long)k->rows + Kv4Part<D>::ROWS - 1) / Kv4Part<D>::ROWS, by = (2l * view.heads + IT - 1) / IT;
     const dim3 grid((unsigned)bx, (unsigned)by);
-    if (READ) k_kv4_read<D, IT><<<grid, 256, 0, (cudaStream_t)stream>>>(view, rows_view(k), rows_view(v));
-    else k_kv4_append<D, IT><<<grid, 256, 0, (cudaStream_t)stream>>>(view, rows_view(k), rows_view(v));
-    return gcuda_check(cudaGetLastError(), what);
+    return attn_launch(what, READ ? k_kv4_read<D, IT> : k_kv4_append<D, IT>, grid, 256, 0, (cudaStream_t)stream, false, view,
+                       rows_view(k), rows_view(v));
 }
 
 // Four items a thread where that still gives every SM two blocks (256 rows of 64

@@ -773,8 +773,7 @@ static int pa_launch(const PromptArgs &a, const ApusHeadRows *q, const ApusHeadR
     CUtensorMap qm, km, vm;
     if (pa_map(&qm, q, D) || pa_map(&km, k, D) || pa_map(&vm, v, D)) return -1;
     if (gcuda_smem_limit_once((const void *)k_prompt_tc<D>, C::SMEM)) return -1;
-    k_prompt_tc<D><<<(unsigned)blocks, C::THREADS, C::SMEM, st>>>(qm, km, vm, a);
-    return gcuda_check(cudaGetLastError(), "prompt_attn launch");
+    return attn_launch("prompt_attn launch", k_prompt_tc<D>, dim3((unsigned)blocks), C::THREADS, C::SMEM, st, false, qm, km, vm, a);
 }
 
 extern "C" int apus_gcuda_prompt_attn_dev(const ApusPromptBatch *batch, const ApusHeadRows *q, const ApusHeadRows *k,

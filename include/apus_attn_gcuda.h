@@ -6,8 +6,9 @@
  *
  * Rules of every entry point here:
  *   - Device pointers, a cudaStream_t passed as void*, the current device.
- *     0 on success; -1 with the reason in apus_gcuda_last_error(), and then
- *     nothing was launched.
+ *     0 on success; -1 with the reason in apus_gcuda_last_error().  Bad
+ *     arguments are refused before anything is launched; where a launch itself
+ *     fails, the outputs are not complete.
  *   - No allocation, no synchronisation, no state kept between calls: every
  *     entry can be captured into a CUDA graph, and calls on different streams
  *     may overlap as long as their outputs and workspaces do not.
