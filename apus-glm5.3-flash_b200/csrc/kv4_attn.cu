@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
         if (s < a.v.nseq) {
             if (!again) {
                 const Kv4Work k = kv4_work(a, s, COLS, 1);
-                if (k.sq.bad && blockIdx.x == 0) atomicMax(&g_kv4a_err, (int)ATTN_ERR_SEQ);
+                if (k.sq.bad && blockIdx.x == 0) atomicExch(&g_kv4a_err, (int)ATTN_ERR_SEQ);
                 per_unit = a.v.heads * k.ncb;
                 pages = (int)k.units;
             }
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                         if (i + lane < mine) {
                             const int page = table[(p0 + (u + lane * kv4::WARPS) * U) / KV4_PAGE];
                             if (kv4_page_ok(page, a.v.num_pages)) my_page = page;
-                            else atomicMax(&g_kv4a_err, (int)ATTN_ERR_PAGE);
+                            else atomicCAS(&g_kv4a_err, 0, (int)ATTN_ERR_PAGE);
                         }
                     }
                     const int page = __shfl_sync(0xffffffffu, my_page, i & 31);
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kv4::THREADS, kv4::resident(NT)) k_kv4_attn(co
                             off[e] = j & (KV4_PAGE - 1);
                             if (kv4_page_ok(page, a.v.num_pages)) src[e] = a.v.pages + kv4_block_at(page, head, a.v.heads, D);
                             else {
-                                atomicMax(&g_kv4a_err, (int)ATTN_ERR_PAGE);
+                                atomicCAS(&g_kv4a_err, 0, (int)ATTN_ERR_PAGE);
                                 list[u0 + r] &= 0xffffu;   // no row sees it
                             }
                         }
@@ -930,7 +930,7 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
             float mx = kv4::NEG_INF, mxl = kv4::NEG_INF;
             // (a lane finds its own pieces' in shared memory again)
             float *const km = kj_dyn, *const kl = kj_dyn + KJ_RUNS, *const kml = kj_dyn + 2 * KJ_RUNS;
-#pragma unroll 4
+#pragma unroll(WIDE ? 4 : 1)
             for (int i = threadIdx.x; i < n; i += 32) {
                 km[i] = piece(i)[cc];
                 kl[i] = piece(i)[cols_block + cc];
@@ -939,12 +939,12 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128, WIDE ? 2 : 12) k_kv4_join(co
             }
 #pragma unroll
             for (int off = 16; off; off >>= 1) mxl = fmaxf(mxl, __shfl_xor_sync(0xffffffffu, mxl, off));
-#pragma unroll 4
+#pragma unroll(WIDE ? 4 : 1)
             for (int i = threadIdx.x; i < n; i += 32) mx = fmaxf(mx, km[i] + (kml[i] - mxl));
 #pragma unroll
             for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
             float sum = 0.f;
-#pragma unroll 4
+#pragma unroll(WIDE ? 4 : 1)
             for (int i = threadIdx.x; i < n; i += 32) {
                 const float mi = km[i], li = kl[i], mli = kml[i];
                 const bool none = mli == kv4::NEG_INF && li == 0.f;

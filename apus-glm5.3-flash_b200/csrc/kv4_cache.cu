@@ -62,7 +62,7 @@ APUS_DEV Kv4Place kv4_place(const Kv4View &v, int row, bool report) {
         pl.page = page;
         pl.off = pos & (KV4_PAGE - 1);
     } else if (report) {
-        atomicMax(&g_kv4_err, (int)ATTN_ERR_PAGE);
+        atomicCAS(&g_kv4_err, 0, (int)ATTN_ERR_PAGE);
     }
     return pl;
 }
@@ -74,7 +74,7 @@ APUS_DEV void kv4_report(const Kv4View &v) {
 #pragma unroll 1
     for (int s = blockIdx.x * 256 + threadIdx.x; s < v.nseq; s += min(gridDim.x, 256) * 256)
         if (kv4_seq(v.cu[s], v.cu[s + 1], v.len[s], v.rows, v.max_rows, v.max_len).bad)
-            atomicMax(&g_kv4_err, (int)ATTN_ERR_SEQ);
+            atomicExch(&g_kv4_err, (int)ATTN_ERR_SEQ);
 }
 
 // Thread -> eight dims (c) of a row; items blockIdx.y * IT .. + IT - 1 of the

@@ -73,7 +73,7 @@ struct PromptSeq { int q0, n, k0, m; };
 APUS_DEV PromptSeq prompt_seq(const PromptArgs &a, int s, bool report) {
     const Kv4Seq q = kv4_seq(a.cu_q[s], a.cu_q[s + 1], 0, a.rows_q, a.max_rows, 0);
     const Kv4Seq k = kv4_seq(a.cu_k[s], a.cu_k[s + 1], 0, a.rows_k, a.rows_k, 0);
-    if ((q.bad || k.bad) && report) atomicMax(&g_pa_err, (int)ATTN_ERR_SEQ);
+    if ((q.bad || k.bad) && report) atomicCAS(&g_pa_err, 0, (int)ATTN_ERR_SEQ);
     return PromptSeq{q.row0, q.n, k.row0, k.n};
 }
 
@@ -364,7 +364,7 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 while (!mbar_try_wait(&clc_full, asked & 1))
                     if (clock64() - t0 > (1ll << 31)) {
                         abort_flag = 1;
-                        atomicMax(&g_pa_err, (int)ATTN_ERR_WAIT);
+                        atomicExch(&g_pa_err, (int)ATTN_ERR_WAIT);
                         ok = false;
                         break;
                     }
