@@ -12,6 +12,10 @@ static_assert(KV4_PAGE == APUS_KV4_PAGE && KV4_GROUP == APUS_KV4_GROUP, "public 
 // took 0.25 us of a short call).
 enum { ATTN_ERR_PAGE = 41, ATTN_ERR_SEQ = 42, ATTN_ERR_WAIT = 43 };
 
+// SMs of a B200, by which work is cut.  A constant: the workspace that a batch needs may
+// be asked for on a host without a GPU, and has to be what the call then uses.
+enum { ATTN_SMS = 148 };
+
 // Device views of the public structs (sizes checked to fit ints).
 struct Kv4View {
     uint8_t *pages;

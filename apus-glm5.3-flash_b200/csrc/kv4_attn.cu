@@ -128,7 +128,7 @@ APUS_DEV int row_of(const Kv4AttnArgs &a, int c) { return (int)(((uint64_t)(uint
 
 APUS_DEV int pool_of(const Kv4AttnArgs &a, int j) { return (int)(((uint64_t)(uint32_t)j * a.pool_magic) >> 36); }
 
-constexpr int KJ_RUNS = 148 * 4;          // runs at most (a multiple of 4)
+constexpr int KJ_RUNS = ATTN_SMS * 4;     // runs at most (a multiple of 4)
 
 // The work: sequence s has heads * ncb segments of `units` units of `unit`
 // pages (one at least, so that a row that sees nothing is written too).
@@ -996,7 +996,7 @@ Kv4Plan kv4_plan(const Kv4View &v, size_t q_heads) {
     const long segs = (long)v.nseq * v.heads * ((cols + 8 * p.nt - 1) / (8 * p.nt));
     p.whole = pages <= WHOLE_PAGES;
     const long most = p.whole ? segs : segs * ((pages + MIN_PAGES - 1) / MIN_PAGES);
-    p.slots = 148 * kv4::resident(p.nt);
+    p.slots = ATTN_SMS * kv4::resident(p.nt);
     p.segs = (int)(segs < p.slots ? segs : p.slots);
     p.grid = (int)(most < p.slots ? most : p.slots);
     p.plan_bytes = ((size_t)v.nseq + 3) * sizeof(long);
@@ -1037,7 +1037,7 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     // form where all blocks are resident at once (131072 positions, 8 segments: 43 us,
     // 47 with the other; 48 sequences, 384 segments: 69 us, 79 with the wide form).
     const long bx = std::min((long)a.group * a.v.max_rows, 64l);
-    const bool wide = bx * a.v.heads * a.v.nseq <= 2 * 148;
+    const bool wide = bx * a.v.heads * a.v.nseq <= 2 * ATTN_SMS;
     return attn_launch("kv4_attn join launch", wide ? k_kv4_join<D, true> : k_kv4_join<D, false>,
                        dim3((unsigned)bx, a.v.heads, a.v.nseq), wide ? 256 : 128, (3 * KJ_RUNS + (wide ? 256 : 128) * 4) * 4, st,
                        true, a, 8 * NT);

@@ -237,7 +237,7 @@ template <int D, bool READ>
 static int kv4_rows_launch(const char *what, const Kv4View &view, const ApusHeadRows *k, const ApusHeadRows *v,
                            void *stream) {
     const long blocks = ((long)k->rows + Kv4Part<D>::ROWS - 1) / Kv4Part<D>::ROWS * ((2l * view.heads + 3) / 4);
-    return blocks >= 2 * 148 ? kv4_rows_launch<D, READ, 4>(what, view, k, v, stream)
+    return blocks >= 2 * ATTN_SMS ? kv4_rows_launch<D, READ, 4>(what, view, k, v, stream)
                              : kv4_rows_launch<D, READ, 2>(what, view, k, v, stream);
 }
 
