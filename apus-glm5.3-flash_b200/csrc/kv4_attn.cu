@@ -4,7 +4,7 @@
 //   z_tj = scale log2(e) q_t . k_j,  m_t = max_j z_tj,
 //   out_t = sum_j 2^(z_tj - m_t) v_j / sum_j 2^(z_tj - m_t)
 //
-// over the visible positions j, in one pass with a running maximum and sum.
+// over the visible positions j, in one pass with running maxima and sums.
 // With k_j = s_jg c_jd and v_j = r_jg e_jd (scale of the group g of 32 dims
 // times an integer code), both contractions run on integer codes:
 //   z_tj  = sum_g s_jg (sum_{d in g} q_td c_jd)
@@ -53,15 +53,19 @@
 // are listed, with a bit for each row that keeps them, and gathered row by row, so
 // what no column keeps is neither read nor computed.
 //
-// Measured (us a call; bytes that it has to read, of 6.55 TB/s): one sequence of
-// 131072 positions, 64 heads over 8 of 128: 41.5 (56%); 48 sequences of up to 8192,
-// 32 over 8: 68.5 (55%); 4 rows over 4363 positions of 64 heads of 256: 31 (39%);
-// 4 rows of 512 pools of 4 out of 32771: 45; 513 positions, 32 over 8: 8.5.  What
-// bounds it is issue: 322 instructions for 16 positions of dim 128 (70 of them LOP3
-// and 20 shifts at half rate: 48% of that pipe, 59% of all issue slots), and about
-// 8 thousand cycles a launch before and after the stream.  A fourth CTA an SM (128
-// registers, the query in shared memory) took 8% longer; two scores an
-// instruction (packed fp32) took 3% off.
+// Measured (us a call in a captured graph; bytes that it has to read, of 6.55 TB/s): one
+// sequence of 131072 positions, 64 heads over 8 of 128: 42.4 (54%); 48 sequences of up
+// to 8192, 32 over 8: 70.7 (53%); 4 rows over 4363 positions of 64 heads of 256: 32
+// (38%); 4 rows of 512 pools of 4 out of 32771: 46; 513 positions, 32 over 8: 8.7.
+// No pipe is full: 334 instructions for 16 positions of dim 128 (812 at dim 256) take
+// 57% of the issue slots in the stream and 48% of the half-rate pipe (LOP3, shifts), and
+// would take 19.5 of the 42.4 us by themselves.  A warp takes 16 positions at a time
+// through one chain (scores, maxima, exponentials, transpose, output), with three warps
+// a scheduler: fixed latencies are the first stall.  About 8 thousand cycles a launch go
+// by before and after the stream.  A fourth CTA an SM (128 registers, the query in shared
+// memory) took 8% longer; two scores an instruction (packed fp32) took 3% off; two
+// fragments in flight a warp have not been tried.  The sum's own maximum and exponentials
+// cost 2 to 4%.
 #include <algorithm>
 #include <type_traits>
 
@@ -87,8 +91,9 @@ template <int D> struct Cfg {
     // pairs of positions, and each position's exponent E
     static constexpr int KF = STAGES * STAGE, VH = KF + U * NG * 4, PW = VH + U * NG * 2;
     static constexpr int WARP_SMEM = PW + U * 4;
-    // the query's fragments, 512 bytes a group: 32 registers at dim 256, which the
-    // loop has not (it spilt); below they stay in registers
+    // the query's fragments, 512 bytes a group: 32 registers at dim 256, which the loop
+    // has not (28 bytes are spilt as it is, and read eight times a warp in a launch);
+    // below they stay in registers
     static constexpr bool QS = D == 256;
     static constexpr int QF = WARPS * WARP_SMEM, SMEM = QF + (QS ? NG * 512 : 0);
 };
@@ -1035,7 +1040,8 @@ int kv4_attn_launch(const Kv4AttnArgs &a, int grid, cudaStream_t st) {
     // the joining kernel starts while the first drains, and waits for it: a block a
     // column, up to 64 (max_rows may be far above the rows that there are).  The wide
     // form where all blocks are resident at once (131072 positions, 8 segments: 43 us,
-    // 47 with the other; 48 sequences, 384 segments: 69 us, 79 with the wide form).
+    // 47 with the other; 48 sequences, 384 segments: 69 us, 79 with the wide form, each
+    // before the sums had maxima of their own).
     const long bx = std::min((long)a.group * a.v.max_rows, 64l);
     const bool wide = bx * a.v.heads * a.v.nseq <= 2 * ATTN_SMS;
     return attn_launch("kv4_attn join launch", wide ? k_kv4_join<D, true> : k_kv4_join<D, false>,

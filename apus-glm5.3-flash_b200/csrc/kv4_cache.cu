@@ -238,7 +238,7 @@ static int kv4_rows_launch(const char *what, const Kv4View &view, const ApusHead
                            void *stream) {
     const long blocks = ((long)k->rows + Kv4Part<D>::ROWS - 1) / Kv4Part<D>::ROWS * ((2l * view.heads + 3) / 4);
     return blocks >= 2 * ATTN_SMS ? kv4_rows_launch<D, READ, 4>(what, view, k, v, stream)
-                             : kv4_rows_launch<D, READ, 2>(what, view, k, v, stream);
+                                  : kv4_rows_launch<D, READ, 2>(what, view, k, v, stream);
 }
 
 template <bool READ>

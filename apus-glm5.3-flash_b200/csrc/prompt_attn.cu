@@ -35,14 +35,17 @@
 // Items: a CTA that is done asks for the item of one that has not begun
 // (clusterlaunchcontrol), so the next item's copies and first products run under
 // the last one's end.  One CTA an item spent 12.7 thousand cycles on set-up, first
-// copies and the end, where 2048 rows of dim 256 take 37 thousand: 172 -> 162 us,
-// seven ragged prompts of dim 128 81 -> 75 us, nine of dim 256 71 -> 62 us.  Heads
+// copies and the end, where 2048 rows of 64 heads of 256 take 37 thousand: 172 -> 162
+// us; seven ragged prompts, 4099 rows of 32 heads over 8 of 128: 81 -> 75 us.  Heads
 // that do not fit L2 together follow one another (L2_SHARE): 162 -> 144 us.
 //
-// Measured: dim 128, 8192 rows after 4096 keys, 32 heads over 8: 0.79 ms, 1380
-// TFLOP/s; dim 256, 8192 rows of 16 heads: 1290 TFLOP/s, 2400 cycles a tile of 2048
-// (a ring of five half tiles in place of four, the same; quarters, V by keys, 730;
-// two softmax groups that take turns, 1160).
+// Measured (captured graphs of a few milliseconds, at 1965 MHz): dim 128, 8192 rows
+// after 4096 keys, 32 heads over 8: 0.79 ms, 1390 TFLOP/s; dim 256, 8192 rows of 16
+// heads: 1290 TFLOP/s, 2400 cycles a tile of 2048 (a ring of five half tiles in place of
+// four, the same; quarters, V by keys, 730; two softmax groups that take turns, 1160);
+// 2048 rows of 64 heads: 139 us, tensor pipe 54% active; dim 64, 8192 rows of 32 heads
+// over 8: 346 us, 794 TFLOP/s.  Over a tenth of a second and more the power limit holds
+// the clock near 1530 MHz: 0.92 ms, and 162 us for the 2048 rows.
 //
 // A hidden key's weight is 0, but 0 times a NaN or an infinity in its value would
 // reach the row through the product.  So in tiles with hidden keys such values
@@ -102,7 +105,8 @@ constexpr float RAISE = 8.0f;
 // Bytes of keys and values that items next to one another read: all items that
 // run at once read them at their own places, so what does not stay in L2 (126 MB)
 // comes from HBM for each block of rows.  64 heads of 256, 2048 rows: 144 us (all
-// heads together, 134 MB: 165; 64 MB 149, 32 MB 144); 4096 rows: 490 (573).
+// heads together, 134 MB: 165; 64 MB 149, 32 MB 144), 4096 rows of the same heads: 490
+// (573), each when this was chosen; 139 and 475 since.
 constexpr int L2_SHARE = 48 << 20;
 }  // namespace pa
 
@@ -632,8 +636,8 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                     for (int c = 0; c < 128; c += 2) f32_unpair(add_f32x2(f32_pair(v[c], v[c + 1]), down), v[c], v[c + 1]);
                     mz = 0.f;
                 }
-                // two scores an instruction (packed fp32): the loop is a quarter shorter (dim 64
-                // 386 -> 357 us, seven ragged prompts 66 -> 63 us)
+                // two scores an instruction (packed fp32): the loop is a quarter shorter (seven
+                // ragged prompts of 32 heads over 8 of 128, 4099 rows: 66 -> 63 us)
                 const uint64_t scale2 = f32_pair(a.zscale, a.zscale), mz2 = f32_pair(-mz, -mz);
                 uint64_t sum[2] = {0, 0};
                 uint32_t pk[2][32];
