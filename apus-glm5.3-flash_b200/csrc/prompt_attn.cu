@@ -630,11 +630,12 @@ k_prompt_tc(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CU
                 float mz = m == -INFINITY ? 0.f : m * a.zscale;
                 // a product that is rounded to 2^-7 and more: the difference first, which is
                 // exact for neighbours (from 2^31 on, the rounding alone reached 2^127)
-                if (__any_sync(0xffffffffu, fabsf(mz) > 65536.0f)) {
-                    const uint64_t down = f32_pair(m == -INFINITY ? 0.f : -m, m == -INFINITY ? 0.f : -m);
+                const bool huge = fabsf(mz) > 65536.0f;      // each row by its own scores alone
+                if (__any_sync(0xffffffffu, huge)) {
+                    const uint64_t down = huge ? f32_pair(-m, -m) : 0;
 #pragma unroll
                     for (int c = 0; c < 128; c += 2) f32_unpair(add_f32x2(f32_pair(v[c], v[c + 1]), down), v[c], v[c + 1]);
-                    mz = 0.f;
+                    if (huge) mz = 0.f;
                 }
                 // two scores an instruction (packed fp32): the loop is a quarter shorter (seven
                 // ragged prompts of 32 heads over 8 of 128, 4099 rows: 66 -> 63 us)

@@ -26,3 +26,20 @@ def test_large_scores(gcuda, dim, group, power):
         got = run(gcuda, q.cuda(), k.cuda(), v.cuda(), [rows], [keys], 1.0).float().cpu()
         held = v[0, 0].float()
         assert ((got - held).abs() <= held.abs() * (2 * R.U + 2.0 ** -16)).all(), (rows, keys)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("big", [2.0 ** 40, float("inf")])
+def test_large_scores_of_other_rows(gcuda, dim, big):
+    """A row's bits do not go by its neighbours' scores, of its own sequence or of the next."""
+    g = gen(dim)
+    rows, keys = [70, 5, 200], [300, 5, 200]
+    q = bf16(g, 275, 2, dim, std=3.0).cuda()
+    k, v = (bf16(g, 505, 1, dim).cuda() for _ in range(2))
+    want = run(gcuda, q, k, v, rows, keys, 0.1)
+    q2 = q.clone()
+    at = [3, 40, 71, 90, 274]
+    q2[at] = (q2[at].float().sign() * big).to(torch.bfloat16)
+    got = run(gcuda, q2, k, v, rows, keys, 0.1)
+    keep = [i for i in range(275) if i not in at]
+    assert torch.equal(got[keep], want[keep])
